@@ -1,0 +1,357 @@
+// Embedding lookup with scaling, and its gradient by sorted tokens.
+//
+// lookup  out[i,:] = round(scale * table[id_i - first,:]), zero where id_i - first
+//         is outside the table (padding, or another rank's part of the vocabulary).
+// grad    dW[v,:] = round(scale * sum of dout[i,:] over id_i - first == v), the sum in
+//         fp32 and in the order of i within a piece of the sorted list, then piece by
+//         piece: the same bits on every run.  Both are bound by HBM bytes.
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "common.cuh"
+#include "index_sort.cuh"
+#include "launch.cuh"
+#include "rowops.cuh"
+
+namespace dcopy {
+namespace {
+
+__device__ __forceinline__ int64_t read_id(const KeySource &k, uint32_t e) {
+  const uint32_t r = k.cols.div(e);
+  const int64_t at = (int64_t)r * k.pitch + (e - r * k.cols.d);
+  return (k.wide ? static_cast<const int64_t *>(k.ids)[at]
+                 : (int64_t)static_cast<const int32_t *>(k.ids)[at]) - k.first;
+}
+
+struct Lookup {
+  void *out;
+  const void *table;
+  int64_t out_pitch, table_pitch;
+  KeySource ids;
+  uint32_t vectors;
+  int lx;
+  float scale;
+};
+
+template <typename TIn, typename TOut, int V, int U>
+__global__ void __launch_bounds__(kRowThreads) lookup_kernel(Lookup p) {
+  pdl_trigger_at_entry();
+  pdl_wait();
+  pdl_launch_dependents();
+  const uint32_t row = blockIdx.x * (kRowThreads >> p.lx) + (threadIdx.x >> p.lx);
+  if (row >= p.ids.n) return;
+  const uint32_t step = 1u << p.lx;
+  const uint32_t c0 = (blockIdx.y * U << p.lx) + (threadIdx.x & (step - 1));
+  const int64_t id = read_id(p.ids, row);
+  const bool known = id >= 0 && id < (int64_t)p.ids.keys;
+  const TIn *src = static_cast<const TIn *>(p.table) + (known ? id * p.table_pitch : 0);
+  TOut *dst = static_cast<TOut *>(p.out) + row * p.out_pitch;
+  Vec<TIn, V> in[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const uint32_t c = c0 + u * step;
+    if (known && c < p.vectors) in[u].load(src + (uint64_t)c * V);
+    else in[u].zero();
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const uint32_t c = c0 + u * step;
+    float f[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = known ? in[u].get(i) * p.scale : 0.0f;
+    Vec<TOut, V> out;
+    out.put(f);
+    if (c < p.vectors) out.store(dst + (uint64_t)c * V);
+  }
+}
+
+// ---- gradient -------------------------------------------------------------------
+
+constexpr uint32_t kPiece = 32;  // sorted entries that one block sums
+
+struct Grad {
+  void *grad;
+  const void *dout;
+  int64_t grad_pitch, dout_pitch;
+  const uint32_t *key, *pos;  // in key order
+  float *head, *tail;         // [pieces][width] sums of runs that cross piece ends
+  uint32_t n, keys, pieces, vectors, width;
+  int lx;
+  float scale;
+};
+
+template <typename T, int V, bool kAdd>
+__device__ __forceinline__ void write_row(T *row, uint32_t c, const float (&sum)[V], float scale) {
+  float f[V];
+  Vec<T, V> old;
+  if constexpr (kAdd) old.load_plain(row + (uint64_t)c * V);
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    f[i] = sum[i] * scale;
+    if constexpr (kAdd) f[i] += old.get(i);
+  }
+  Vec<T, V> out;
+  out.put(f);
+  out.store(row + (uint64_t)c * V);
+}
+
+// One piece of the sorted list: runs of equal ids that lie inside it are summed and
+// written; what a run that crosses an end of the piece has here goes to head (it
+// began earlier) or tail (it begins here and goes on).
+template <typename TIn, typename TOut, int V, bool kAdd>
+__global__ void __launch_bounds__(kRowThreads) piece_sum_kernel(Grad p) {
+  pdl_trigger_at_entry();
+  pdl_wait();
+  pdl_launch_dependents();
+  const uint32_t piece = blockIdx.x * (kRowThreads >> p.lx) + (threadIdx.x >> p.lx);
+  const uint32_t c = (blockIdx.y << p.lx) + (threadIdx.x & ((1u << p.lx) - 1));
+  if (piece >= p.pieces || c >= p.vectors) return;
+  const uint32_t b = piece * kPiece, e = min(b + kPiece, p.n);
+  const TIn *dout = static_cast<const TIn *>(p.dout) + (uint64_t)c * V;
+  TOut *grad = static_cast<TOut *>(p.grad);
+  uint32_t key = p.key[b];
+  bool open = b > 0 && p.key[b - 1] == key;  // the run began in an earlier piece
+  float sum[V] = {};
+  constexpr int kAhead = 4;
+  for (uint32_t i0 = b; i0 < e && key < p.keys; i0 += kAhead) {
+    Vec<TIn, V> in[kAhead];
+    uint32_t next[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const uint32_t i = i0 + j;
+      if (i < e) in[j].load(dout + (int64_t)p.pos[i] * p.dout_pitch);
+      next[j] = i + 1 < p.n ? p.key[i + 1] : p.keys;
+    }
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      if (i0 + j >= e || key >= p.keys) break;
+#pragma unroll
+      for (int v = 0; v < V; ++v) sum[v] += in[j].get(v);
+      if (next[j] != key || i0 + j + 1 == e) {
+        float *part = open ? p.head : next[j] == key ? p.tail : nullptr;
+        if (part) {
+          Vec<float, V> out;
+          out.put(sum);
+          out.store(part + (uint64_t)piece * p.width + (uint64_t)c * V);
+        } else {
+          write_row<TOut, V, kAdd>(grad + key * p.grad_pitch, c, sum, p.scale);
+        }
+#pragma unroll
+        for (int v = 0; v < V; ++v) sum[v] = 0.0f;
+        open = false;
+        key = next[j];
+      }
+    }
+  }
+}
+
+// The runs that begin in a piece and go on: tail of that piece plus the heads of the
+// following ones, in order.
+template <typename TOut, int V, bool kAdd>
+__global__ void __launch_bounds__(kRowThreads) piece_join_kernel(Grad p) {
+  pdl_trigger_at_entry();
+  pdl_wait();
+  pdl_launch_dependents();
+  const uint32_t piece = blockIdx.x * (kRowThreads >> p.lx) + (threadIdx.x >> p.lx);
+  const uint32_t c = (blockIdx.y << p.lx) + (threadIdx.x & ((1u << p.lx) - 1));
+  if (piece + 1 >= p.pieces || c >= p.vectors) return;
+  const uint32_t b = piece * kPiece, last = b + kPiece - 1;
+  const uint32_t key = p.key[last];
+  if (key >= p.keys || p.key[last + 1] != key) return;    // nothing goes on
+  if (p.key[b] == key && b > 0 && p.key[b - 1] == key) return;  // it began earlier
+  const uint64_t at = (uint64_t)c * V;
+  float sum[V];
+  Vec<float, V> part;
+  part.load(p.tail + (uint64_t)piece * p.width + at);
+#pragma unroll
+  for (int v = 0; v < V; ++v) sum[v] = part.get(v);
+  for (uint32_t q = piece + 1; q < p.pieces && p.key[q * kPiece] == key; ++q) {
+    part.load(p.head + (uint64_t)q * p.width + at);
+#pragma unroll
+    for (int v = 0; v < V; ++v) sum[v] += part.get(v);
+  }
+  write_row<TOut, V, kAdd>(static_cast<TOut *>(p.grad) + key * p.grad_pitch, c, sum, p.scale);
+}
+
+// Zeroes rows of `bytes` bytes, `pitch` bytes apart, in units of N bytes.
+template <int N>
+__global__ void __launch_bounds__(kRowThreads) zero_rows_kernel(uint8_t *dst, uint64_t pitch,
+                                                                uint64_t units, uint32_t rows) {
+  pdl_trigger_at_entry();
+  pdl_wait();
+  pdl_launch_dependents();
+  Words<N> z;
+  z.zero();
+  for (uint32_t r = blockIdx.y; r < rows; r += gridDim.y)
+    for (uint64_t c = (uint64_t)blockIdx.x * kRowThreads + threadIdx.x; c < units;
+         c += (uint64_t)gridDim.x * kRowThreads)
+      z.store(dst + r * pitch + c * N);
+}
+
+int zero_rows(const DcopyMatrix *m, cudaStream_t s) {
+  const int eb = elem_size(m->type);
+  uint64_t rows = m->rows, bytes = (uint64_t)m->cols * eb;
+  const uint64_t pitch = (uint64_t)m->pitch * eb;
+  if (rows <= 1 || pitch == bytes) bytes *= rows, rows = 1;
+  const uint64_t all = (uintptr_t)m->data | bytes | (rows > 1 ? pitch : 0);
+  const int unit = all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 2;
+  const uint64_t units = bytes / unit;
+  const uint64_t gy = std::min<uint64_t>(rows, 65535);
+  const uint64_t most = (uint64_t)sm_count() * 32;
+  const uint64_t gx = std::min<uint64_t>((units + kRowThreads - 1) / kRowThreads,
+                                         std::max<uint64_t>(1, most / gy));
+  auto k = unit == 16 ? zero_rows_kernel<16> : unit == 4 ? zero_rows_kernel<4> : zero_rows_kernel<2>;
+  return launch_grid(k, dim3((unsigned)gx, (unsigned)gy), dim3(kRowThreads), 0, s,
+                     "zero_rows_kernel", static_cast<uint8_t *>(m->data), pitch, units,
+                     (uint32_t)rows);
+}
+
+int id_source(const DcopyMatrix *ids, int64_t first, int64_t keys, KeySource *src) {
+  if (int rc = check_matrix(ids, "ids", is_index(ids->type))) return rc;
+  const uint64_t n = (uint64_t)ids->rows * (uint64_t)ids->cols;
+  if (n > INT32_MAX)
+    return set_error(DCOPY_ERR_SHAPE_INVALID, "ids: %llu entries", (unsigned long long)n);
+  src->ids = ids->data;
+  src->pitch = ids->pitch;
+  src->first = first;
+  src->keys = (uint32_t)keys;
+  src->wide = ids->type == kI64;
+  src->n = (uint32_t)n;
+  src->cols = FastDiv((uint32_t)std::max<int64_t>(1, ids->cols));
+  return DCOPY_OK;
+}
+
+uint64_t pieces_of(uint64_t n) { return (n + kPiece - 1) / kPiece; }
+
+}  // namespace
+}  // namespace dcopy
+
+using namespace dcopy;
+
+extern "C" {
+
+int dcopy_embedding_lookup(const DcopyMatrix *out, const DcopyMatrix *table,
+                           const DcopyMatrix *ids, int64_t first_id, float scale,
+                           dcopy_stream_t stream) {
+  DCOPY_API_BEGIN
+  if (!out || !table || !ids)
+    return set_error(DCOPY_ERR_PARAM_INVALID, "embedding_lookup: NULL matrix");
+  if (int rc = check_matrix(out, "out", is_float(out->type))) return rc;
+  if (int rc = check_matrix(table, "table", is_float(table->type))) return rc;
+  Lookup p{};
+  if (int rc = id_source(ids, first_id, table->rows, &p.ids)) return rc;
+  if (out->rows != (int64_t)p.ids.n || out->cols != table->cols)
+    return set_error(DCOPY_ERR_SHAPE_INVALID,
+                     "embedding_lookup: out is %lld x %lld for %u ids and a table of width %lld",
+                     (long long)out->rows, (long long)out->cols, p.ids.n, (long long)table->cols);
+  if (out->cols > kMaxWidth)
+    return set_error(DCOPY_ERR_UNSUPPORTED, "embedding_lookup: width %lld", (long long)out->cols);
+  if (out->rows == 0 || out->cols == 0) return DCOPY_OK;
+  if (int rc = check_apart(out, table, "embedding_lookup")) return rc;
+  if (int rc = check_apart(out, ids, "embedding_lookup")) return rc;
+  p.out = out->data;
+  p.table = table->data;
+  p.out_pitch = out->pitch;
+  p.table_pitch = table->pitch;
+  p.scale = scale;
+  return with_float(table->type, [&](auto tin) {
+    return with_float(out->type, [&](auto tout) {
+      using TIn = typename decltype(tin)::type;
+      using TOut = typename decltype(tout)::type;
+      return with_vector(std::min(vector_width(out), vector_width(table)), [&](auto vw) {
+        constexpr int V = decltype(vw)::value;
+        p.vectors = (uint32_t)(out->cols / V);
+        const bool many = (uint64_t)p.ids.n * p.vectors >= (uint64_t)sm_count() * 2048 * 4;
+        const RowSplit split = split_rows(p.ids.n, p.vectors, many ? 4 : 1);
+        p.lx = split.lx;
+        auto k = many ? lookup_kernel<TIn, TOut, V, 4> : lookup_kernel<TIn, TOut, V, 1>;
+        return launch_grid(k, split.grid, dim3(kRowThreads), 0, stream, "lookup_kernel", p);
+      });
+    });
+  });
+  DCOPY_API_END
+}
+
+int dcopy_embedding_grad_workspace(int64_t tokens, int64_t vocab, int64_t width,
+                                   uint64_t *bytes) {
+  DCOPY_API_BEGIN
+  if (!bytes || tokens < 0 || vocab < 0 || width < 0 || tokens > INT32_MAX || vocab > INT32_MAX ||
+      width > kMaxWidth)
+    return set_error(DCOPY_ERR_PARAM_INVALID, "embedding_grad_workspace: %lld tokens, %lld x %lld",
+                     (long long)tokens, (long long)vocab, (long long)width);
+  const uint64_t sort = (sort_by_key_bytes(tokens, vocab) + 15) / 16 * 16;
+  const uint64_t row = ((uint64_t)width * sizeof(float) + 15) / 16 * 16;
+  *bytes = sort + 2 * pieces_of(tokens) * row + 32;
+  return DCOPY_OK;
+  DCOPY_API_END
+}
+
+int dcopy_embedding_grad(const DcopyMatrix *grad, const DcopyMatrix *dout, const DcopyMatrix *ids,
+                         int64_t first_id, float scale, int32_t accumulate, void *workspace,
+                         uint64_t workspace_bytes, dcopy_stream_t stream) {
+  DCOPY_API_BEGIN
+  if (!grad || !dout || !ids)
+    return set_error(DCOPY_ERR_PARAM_INVALID, "embedding_grad: NULL matrix");
+  if (int rc = check_matrix(grad, "grad", is_float(grad->type))) return rc;
+  if (int rc = check_matrix(dout, "dout", is_float(dout->type))) return rc;
+  KeySource src{};
+  if (int rc = id_source(ids, first_id, grad->rows, &src)) return rc;
+  if (dout->rows != (int64_t)src.n || dout->cols != grad->cols)
+    return set_error(DCOPY_ERR_SHAPE_INVALID,
+                     "embedding_grad: dout is %lld x %lld for %u ids and a table of width %lld",
+                     (long long)dout->rows, (long long)dout->cols, src.n, (long long)grad->cols);
+  if (grad->cols > kMaxWidth)
+    return set_error(DCOPY_ERR_UNSUPPORTED, "embedding_grad: width %lld", (long long)grad->cols);
+  uint64_t need = 0;
+  if (int rc = dcopy_embedding_grad_workspace(src.n, grad->rows, grad->cols, &need)) return rc;
+  if (src.n && workspace_bytes < need)
+    return set_error(DCOPY_ERR_PARAM_INVALID, "embedding_grad: workspace of %llu bytes, %llu needed",
+                     (unsigned long long)workspace_bytes, (unsigned long long)need);
+  if (src.n)
+    if (int rc = check_device_span(workspace, need, "workspace")) return rc;
+  if (int rc = check_apart(grad, dout, "embedding_grad")) return rc;
+  if (int rc = check_apart(grad, ids, "embedding_grad")) return rc;
+  if (grad->rows == 0 || grad->cols == 0) return DCOPY_OK;
+  if (!accumulate)
+    if (int rc = zero_rows(grad, stream)) return rc;
+  if (src.n == 0) return DCOPY_OK;
+  uint8_t *ws = reinterpret_cast<uint8_t *>(((uintptr_t)workspace + 15) / 16 * 16);
+  const uint64_t sort = (sort_by_key_bytes(src.n, grad->rows) + 15) / 16 * 16;
+  Grad p{};
+  if (int rc = sort_by_key(src, ws, &p.key, &p.pos, stream)) return rc;
+  p.grad = grad->data;
+  p.dout = dout->data;
+  p.grad_pitch = grad->pitch;
+  p.dout_pitch = dout->pitch;
+  p.n = src.n;
+  p.keys = src.keys;
+  p.pieces = (uint32_t)pieces_of(src.n);
+  p.width = (uint32_t)((grad->cols + 3) / 4 * 4);
+  p.head = reinterpret_cast<float *>(ws + sort);
+  p.tail = p.head + (uint64_t)p.pieces * p.width;
+  p.scale = scale;
+  return with_float(dout->type, [&](auto tin) {
+    return with_float(grad->type, [&](auto tout) {
+      using TIn = typename decltype(tin)::type;
+      using TOut = typename decltype(tout)::type;
+      return with_vector(std::min(vector_width(dout), vector_width(grad)), [&](auto vw) {
+        constexpr int V = decltype(vw)::value;
+        p.vectors = (uint32_t)(grad->cols / V);
+        const RowSplit split = split_rows(p.pieces, p.vectors, 1);
+        p.lx = split.lx;
+        auto sum = accumulate ? piece_sum_kernel<TIn, TOut, V, true>
+                              : piece_sum_kernel<TIn, TOut, V, false>;
+        auto join = accumulate ? piece_join_kernel<TOut, V, true> : piece_join_kernel<TOut, V, false>;
+        if (int rc = launch_grid(sum, split.grid, dim3(kRowThreads), 0, stream, "piece_sum_kernel", p))
+          return rc;
+        if (p.pieces == 1) return DCOPY_OK;
+        return launch_grid(join, split.grid, dim3(kRowThreads), 0, stream, "piece_join_kernel", p);
+      });
+    });
+  });
+  DCOPY_API_END
+}
+
+}  // extern "C"

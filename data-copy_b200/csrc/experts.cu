@@ -1,0 +1,459 @@
+// Tokens sorted by expert and back, with weights, and the gradient.
+//
+// sort      the entries (token i, slot j) in expert order, the earlier first:
+//           dest[i,j] = row of the entry, source[row] = i * slots + j
+// dispatch  out[dest[i,j],:] = (w[i,j] *) x[i,:], rows without an entry are zeroed
+// combine   out[i,:] = round(sum over j of (w[i,j] *) y[dest[i,j],:]), in fp32, j ascending
+// combine_grad  dy[dest[i,j],:] = round(w[i,j] * dout[i,:]),
+//           dw[i,j] = sum over the columns of dout[i,:] * y[dest[i,j],:]
+// All are bound by the bytes of the rows: each row is read once and written once.
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "common.cuh"
+#include "index_sort.cuh"
+#include "launch.cuh"
+#include "rowops.cuh"
+
+namespace dcopy {
+namespace {
+
+struct Route {
+  void *out;              // dispatch: rows in expert order; combine: tokens
+  const void *in;         // dispatch: tokens; combine: rows in expert order
+  const void *dout;       // combine_grad: tokens
+  float *dweights;
+  int64_t out_pitch, in_pitch, dout_pitch, w_pitch, dw_pitch;
+  const int32_t *dest, *source;
+  const float *weights;
+  uint32_t tokens, slots, rows, vectors, token_blocks;
+  int lx;
+};
+
+// Rows of the buffer in expert order that hold no entry are zeroed: this part of
+// the grid looks at kRowThreads rows a block.
+template <int N>
+__device__ __forceinline__ void zero_unused(const Route &p, uint32_t block, void *rows) {
+  const uint32_t lane = threadIdx.x & 31;
+  const uint32_t r = block * kRowThreads + threadIdx.x;
+  uint32_t empty = __ballot_sync(~0u, r < p.rows && p.source[r] < 0);
+  Words<N> z;
+  z.zero();
+  for (; empty; empty &= empty - 1) {
+    const uint32_t row = (r & ~31u) + __ffs(empty) - 1;
+    uint8_t *at = static_cast<uint8_t *>(rows) + row * p.out_pitch;
+    for (uint32_t c = blockIdx.y * 32 + lane; c < p.vectors; c += gridDim.y * 32)
+      z.store(at + (uint64_t)c * N);
+  }
+}
+
+// Rows moved as N-byte units; pitches in bytes.
+template <int N, int U>
+__global__ void __launch_bounds__(kRowThreads) dispatch_kernel(Route p) {
+  pdl_trigger_at_entry();
+  pdl_wait();
+  pdl_launch_dependents();
+  if (blockIdx.x >= p.token_blocks) return zero_unused<N>(p, blockIdx.x - p.token_blocks, p.out);
+  const uint32_t token = blockIdx.x * (kRowThreads >> p.lx) + (threadIdx.x >> p.lx);
+  if (token >= p.tokens) return;
+  const uint32_t step = 1u << p.lx;
+  const uint32_t c0 = (blockIdx.y * U << p.lx) + (threadIdx.x & (step - 1));
+  const uint8_t *src = static_cast<const uint8_t *>(p.in) + token * p.in_pitch;
+  Words<N> in[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (c0 + u * step < p.vectors) in[u].load(src + (uint64_t)(c0 + u * step) * N);
+  const int32_t *dest = p.dest + (uint64_t)token * p.slots;
+  for (uint32_t j = 0; j < p.slots; ++j) {
+    const int32_t row = dest[j];
+    if (row < 0 || (uint32_t)row >= p.rows) continue;
+    uint8_t *dst = static_cast<uint8_t *>(p.out) + row * p.out_pitch;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (c0 + u * step < p.vectors) in[u].store(dst + (uint64_t)(c0 + u * step) * N);
+  }
+}
+
+// The same with a factor for each entry; pitches in elements, as below.
+template <typename T, int V>
+__global__ void __launch_bounds__(kRowThreads) dispatch_weighted_kernel(Route p) {
+  pdl_trigger_at_entry();
+  pdl_wait();
+  pdl_launch_dependents();
+  if (blockIdx.x >= p.token_blocks) {
+    p.out_pitch *= sizeof(T);
+    return zero_unused<(int)sizeof(T) * V>(p, blockIdx.x - p.token_blocks, p.out);
+  }
+  const uint32_t token = blockIdx.x * (kRowThreads >> p.lx) + (threadIdx.x >> p.lx);
+  const uint32_t c = (blockIdx.y << p.lx) + (threadIdx.x & ((1u << p.lx) - 1));
+  if (token >= p.tokens || c >= p.vectors) return;
+  Vec<T, V> in;
+  in.load(static_cast<const T *>(p.in) + token * p.in_pitch + (uint64_t)c * V);
+  for (uint32_t j = 0; j < p.slots; ++j) {
+    const int32_t row = p.dest[(uint64_t)token * p.slots + j];
+    if (row < 0 || (uint32_t)row >= p.rows) continue;
+    const float w = p.weights[token * p.w_pitch + j];
+    float f[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = in.get(i) * w;
+    Vec<T, V> out;
+    out.put(f);
+    out.store(static_cast<T *>(p.out) + row * p.out_pitch + (uint64_t)c * V);
+  }
+}
+
+template <typename T, int V>
+__global__ void __launch_bounds__(kRowThreads) combine_kernel(Route p) {
+  pdl_trigger_at_entry();
+  pdl_wait();
+  pdl_launch_dependents();
+  const uint32_t token = blockIdx.x * (kRowThreads >> p.lx) + (threadIdx.x >> p.lx);
+  const uint32_t c = (blockIdx.y << p.lx) + (threadIdx.x & ((1u << p.lx) - 1));
+  if (token >= p.tokens || c >= p.vectors) return;
+  const T *rows = static_cast<const T *>(p.in) + (uint64_t)c * V;
+  float sum[V] = {};
+  constexpr int kAhead = 4;
+  for (uint32_t j0 = 0; j0 < p.slots; j0 += kAhead) {
+    Vec<T, V> in[kAhead];
+    float w[kAhead];
+    bool kept[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const bool there = j0 + j < p.slots;
+      const int32_t row = there ? p.dest[(uint64_t)token * p.slots + j0 + j] : -1;
+      kept[j] = row >= 0 && (uint32_t)row < p.rows;
+      w[j] = 1.0f;
+      if (kept[j]) {
+        in[j].load(rows + row * p.in_pitch);
+        if (p.weights) w[j] = p.weights[token * p.w_pitch + j0 + j];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+      if (kept[j]) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) sum[i] = fmaf(w[j], in[j].get(i), sum[i]);
+      }
+  }
+  Vec<T, V> out;
+  out.put(sum);
+  out.store(static_cast<T *>(p.out) + token * p.out_pitch + (uint64_t)c * V);
+}
+
+// A block takes a token: its dout row meets each of the token's rows of y.
+template <typename T, int V>
+__global__ void __launch_bounds__(kRowThreads) combine_grad_kernel(Route p) {
+  __shared__ float part[kRowThreads / 32];
+  pdl_trigger_at_entry();
+  pdl_wait();
+  pdl_launch_dependents();
+  if (blockIdx.x >= p.token_blocks) {
+    p.out_pitch *= sizeof(T);
+    return zero_unused<(int)sizeof(T) * V>(p, blockIdx.x - p.token_blocks, p.out);
+  }
+  const uint32_t token = blockIdx.x;
+  const T *dout = static_cast<const T *>(p.dout) + token * p.dout_pitch;
+  for (uint32_t j = 0; j < p.slots; ++j) {
+    const int32_t row = p.dest[(uint64_t)token * p.slots + j];
+    const bool kept = row >= 0 && (uint32_t)row < p.rows;
+    float dot = 0.0f;
+    if (kept) {
+      const float w = p.weights[token * p.w_pitch + j];
+      const T *y = static_cast<const T *>(p.in) + row * p.in_pitch;
+      T *dy = static_cast<T *>(p.out) + row * p.out_pitch;
+      for (uint32_t c = threadIdx.x; c < p.vectors; c += blockDim.x) {
+        Vec<T, V> g, in, out;
+        g.load(dout + (uint64_t)c * V);
+        in.load(y + (uint64_t)c * V);
+        float f[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float d = g.get(i);
+          dot = fmaf(d, in.get(i), dot);
+          f[i] = d * w;
+        }
+        out.put(f);
+        out.store(dy + (uint64_t)c * V);
+      }
+    }
+#pragma unroll
+    for (int o = 16; o; o /= 2) dot += __shfl_xor_sync(~0u, dot, o);
+    if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = dot;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      float all = 0.0f;
+      for (uint32_t w = 0; w < blockDim.x / 32; ++w) all += part[w];
+      p.dweights[token * p.dw_pitch + j] = all;
+    }
+    __syncthreads();
+  }
+}
+
+int check_route(const int32_t *dest, int64_t tokens, int64_t slots, const int32_t *source,
+                int64_t rows, const DcopyMatrix *weights, const char *what) {
+  if (slots < 0 || slots > INT32_MAX ||
+      (unsigned __int128)tokens * (uint64_t)slots > (uint64_t)INT32_MAX)
+    return set_error(DCOPY_ERR_SHAPE_INVALID, "%s: %lld tokens x %lld slots", what,
+                     (long long)tokens, (long long)slots);
+  const uint64_t n = (uint64_t)tokens * slots;
+  if (int rc = check_device_span(dest, n * 4, "dest")) return rc;
+  if (source)
+    if (int rc = check_device_span(source, (uint64_t)rows * 4, "source")) return rc;
+  if (weights) {
+    if (int rc = check_matrix(weights, "weights", weights->type == kF32)) return rc;
+    if (weights->rows != tokens || weights->cols != slots)
+      return set_error(DCOPY_ERR_SHAPE_INVALID, "%s: weights are %lld x %lld, not %lld x %lld",
+                       what, (long long)weights->rows, (long long)weights->cols,
+                       (long long)tokens, (long long)slots);
+  }
+  return DCOPY_OK;
+}
+
+int check_width(const DcopyMatrix *a, const DcopyMatrix *b, const char *what) {
+  if (a->type != b->type)
+    return set_error(DCOPY_ERR_DATATYPE_INVALID, "%s: element types %d and %d differ", what,
+                     a->type, b->type);
+  if (a->cols != b->cols)
+    return set_error(DCOPY_ERR_SHAPE_INVALID, "%s: widths %lld and %lld differ", what,
+                     (long long)a->cols, (long long)b->cols);
+  if (a->cols > kMaxWidth)
+    return set_error(DCOPY_ERR_UNSUPPORTED, "%s: width %lld", what, (long long)a->cols);
+  return DCOPY_OK;
+}
+
+uint32_t unused_blocks(const int32_t *source, uint64_t rows) {
+  return source ? (uint32_t)((rows + kRowThreads - 1) / kRowThreads) : 0;
+}
+
+}  // namespace
+}  // namespace dcopy
+
+using namespace dcopy;
+
+extern "C" {
+
+int dcopy_expert_rows(int64_t entries, int32_t experts, int32_t align, int64_t *rows) {
+  DCOPY_API_BEGIN
+  if (!rows || entries < 0 || experts < 1 || align < 1)
+    return set_error(DCOPY_ERR_PARAM_INVALID, "expert_rows: %lld entries, %d experts, align %d",
+                     (long long)entries, experts, align);
+  if (entries > INT32_MAX)
+    return set_error(DCOPY_ERR_SHAPE_INVALID, "expert_rows: %lld entries", (long long)entries);
+  const int64_t r = entries + std::min<int64_t>(experts, entries) * (align - 1);
+  if (r > INT32_MAX)
+    return set_error(DCOPY_ERR_SHAPE_INVALID, "expert_rows: %lld rows", (long long)r);
+  *rows = r;
+  return DCOPY_OK;
+  DCOPY_API_END
+}
+
+int dcopy_expert_sort_workspace(int64_t entries, int32_t experts, uint64_t *bytes) {
+  DCOPY_API_BEGIN
+  if (experts > (int32_t)kMaxExperts)
+    return set_error(DCOPY_ERR_UNSUPPORTED, "expert_sort_workspace: %d experts (at most %u)",
+                     experts, kMaxExperts);
+  if (!bytes || entries < 0 || entries > INT32_MAX || experts < 1)
+    return set_error(DCOPY_ERR_PARAM_INVALID, "expert_sort_workspace: %lld entries, %d experts",
+                     (long long)entries, experts);
+  *bytes = sort_experts_bytes(entries, experts) + 16;
+  return DCOPY_OK;
+  DCOPY_API_END
+}
+
+int dcopy_expert_sort(int32_t *dest, int32_t *source, int64_t rows, int32_t *offsets,
+                      const DcopyMatrix *expert_ids, int32_t experts, int32_t align,
+                      void *workspace, uint64_t workspace_bytes, dcopy_stream_t stream) {
+  DCOPY_API_BEGIN
+  if (!expert_ids) return set_error(DCOPY_ERR_PARAM_INVALID, "expert_sort: NULL matrix");
+  if (experts < 1 || align < 1)
+    return set_error(DCOPY_ERR_PARAM_INVALID, "expert_sort: %d experts, align %d", experts, align);
+  if (experts > (int32_t)kMaxExperts)
+    return set_error(DCOPY_ERR_UNSUPPORTED, "expert_sort: %d experts (at most %u)", experts,
+                     kMaxExperts);
+  if (int rc = check_matrix(expert_ids, "expert_ids", is_index(expert_ids->type))) return rc;
+  const uint64_t n = (uint64_t)expert_ids->rows * (uint64_t)expert_ids->cols;
+  if (n > INT32_MAX)
+    return set_error(DCOPY_ERR_SHAPE_INVALID, "expert_sort: %llu entries", (unsigned long long)n);
+  int64_t least = 0;
+  if (int rc = dcopy_expert_rows((int64_t)n, experts, align, &least)) return rc;
+  if (rows < least || rows > INT32_MAX)
+    return set_error(DCOPY_ERR_SHAPE_INVALID, "expert_sort: source has %lld rows, %lld needed",
+                     (long long)rows, (long long)least);
+  const uint64_t need = sort_experts_bytes(n, (uint32_t)experts);
+  if (need && workspace_bytes < need + 16)
+    return set_error(DCOPY_ERR_PARAM_INVALID, "expert_sort: workspace of %llu bytes, %llu needed",
+                     (unsigned long long)workspace_bytes, (unsigned long long)need + 16);
+  if (int rc = check_device_span(dest, n * 4, "dest")) return rc;
+  if (int rc = check_device_span(source, (uint64_t)rows * 4, "source")) return rc;
+  if (int rc = check_device_span(offsets, ((uint64_t)experts + 1) * 4, "offsets")) return rc;
+  if (need)
+    if (int rc = check_device_span(workspace, need + 16, "workspace")) return rc;
+  KeySource src{};
+  src.ids = expert_ids->data;
+  src.pitch = expert_ids->pitch;
+  src.keys = (uint32_t)experts;
+  src.wide = expert_ids->type == kI64;
+  src.n = (uint32_t)n;
+  src.cols = FastDiv((uint32_t)std::max<int64_t>(1, expert_ids->cols));
+  void *ws = reinterpret_cast<void *>(((uintptr_t)workspace + 15) / 16 * 16);
+  return sort_experts(src, (uint32_t)align, dest, source, (uint32_t)rows, offsets, ws, stream);
+  DCOPY_API_END
+}
+
+int dcopy_expert_dispatch(const DcopyMatrix *out, const DcopyMatrix *x, const int32_t *dest,
+                          int64_t slots, const int32_t *source, const DcopyMatrix *weights,
+                          dcopy_stream_t stream) {
+  DCOPY_API_BEGIN
+  if (!out || !x) return set_error(DCOPY_ERR_PARAM_INVALID, "expert_dispatch: NULL matrix");
+  if (int rc = check_matrix(out, "out", weights ? is_float(out->type) : elem_size(out->type) > 0))
+    return rc;
+  if (int rc = check_matrix(x, "x", weights ? is_float(x->type) : elem_size(x->type) > 0))
+    return rc;
+  if (int rc = check_width(out, x, "expert_dispatch")) return rc;
+  if (int rc = check_route(dest, x->rows, slots, source, out->rows, weights, "expert_dispatch"))
+    return rc;
+  if (int rc = check_apart(out, x, "expert_dispatch")) return rc;
+  if (out->rows == 0 || out->cols == 0) return DCOPY_OK;
+  Route p{};
+  p.out = out->data;
+  p.in = x->data;
+  p.dest = dest;
+  p.source = source;
+  p.tokens = (uint32_t)x->rows;
+  p.slots = (uint32_t)slots;
+  p.rows = (uint32_t)out->rows;
+  if (weights) {
+    p.weights = static_cast<const float *>(weights->data);
+    p.w_pitch = weights->pitch;
+    p.out_pitch = out->pitch;
+    p.in_pitch = x->pitch;
+    return with_float(out->type, [&](auto t) {
+      using T = typename decltype(t)::type;
+      return with_vector(std::min(vector_width(out), vector_width(x)), [&](auto vw) {
+        constexpr int V = decltype(vw)::value;
+        p.vectors = (uint32_t)(out->cols / V);
+        RowSplit split = split_rows(p.tokens, p.vectors, 1);
+        p.lx = split.lx;
+        p.token_blocks = split.grid.x;
+        split.grid.x += unused_blocks(source, out->rows);
+        if (split.grid.x == 0) return (int)DCOPY_OK;
+        return launch_grid(dispatch_weighted_kernel<T, V>, split.grid, dim3(kRowThreads), 0, stream,
+                           "dispatch_weighted_kernel", p);
+      });
+    });
+  }
+  const int eb = elem_size(out->type);
+  p.out_pitch = out->pitch * eb;
+  p.in_pitch = x->pitch * eb;
+  const uint64_t bytes = (uint64_t)out->cols * eb;
+  const uint64_t all = (uintptr_t)out->data | (uintptr_t)x->data | bytes |
+                       (out->rows > 1 ? p.out_pitch : 0) | (x->rows > 1 ? p.in_pitch : 0);
+  const int unit = all % 16 == 0 ? 16 : all % 8 == 0 ? 8 : all % 4 == 0 ? 4 : all % 2 == 0 ? 2 : 1;
+  p.vectors = (uint32_t)(bytes / unit);
+  RowSplit split = split_rows(p.tokens, p.vectors, 1);
+  p.lx = split.lx;
+  p.token_blocks = split.grid.x;
+  split.grid.x += unused_blocks(source, out->rows);
+  if (split.grid.x == 0) return DCOPY_OK;
+  auto k = unit == 16 ? dispatch_kernel<16, 1> : unit == 8 ? dispatch_kernel<8, 1>
+           : unit == 4 ? dispatch_kernel<4, 1> : unit == 2 ? dispatch_kernel<2, 1>
+                                                           : dispatch_kernel<1, 1>;
+  return launch_grid(k, split.grid, dim3(kRowThreads), 0, stream, "dispatch_kernel", p);
+  DCOPY_API_END
+}
+
+int dcopy_expert_combine(const DcopyMatrix *out, const DcopyMatrix *y, const int32_t *dest,
+                         int64_t slots, const DcopyMatrix *weights, dcopy_stream_t stream) {
+  DCOPY_API_BEGIN
+  if (!out || !y) return set_error(DCOPY_ERR_PARAM_INVALID, "expert_combine: NULL matrix");
+  if (int rc = check_matrix(out, "out", is_float(out->type))) return rc;
+  if (int rc = check_matrix(y, "y", is_float(y->type))) return rc;
+  if (int rc = check_width(out, y, "expert_combine")) return rc;
+  if (int rc = check_route(dest, out->rows, slots, nullptr, 0, weights, "expert_combine")) return rc;
+  if (int rc = check_apart(out, y, "expert_combine")) return rc;
+  if (out->rows == 0 || out->cols == 0) return DCOPY_OK;
+  Route p{};
+  p.out = out->data;
+  p.in = y->data;
+  p.out_pitch = out->pitch;
+  p.in_pitch = y->pitch;
+  p.dest = dest;
+  if (weights) {
+    p.weights = static_cast<const float *>(weights->data);
+    p.w_pitch = weights->pitch;
+  }
+  p.tokens = (uint32_t)out->rows;
+  p.slots = (uint32_t)slots;
+  p.rows = (uint32_t)y->rows;
+  return with_float(out->type, [&](auto t) {
+    using T = typename decltype(t)::type;
+    return with_vector(std::min(vector_width(out), vector_width(y)), [&](auto vw) {
+      constexpr int V = decltype(vw)::value;
+      p.vectors = (uint32_t)(out->cols / V);
+      const RowSplit split = split_rows(p.tokens, p.vectors, 1);
+      p.lx = split.lx;
+      return launch_grid(combine_kernel<T, V>, split.grid, dim3(kRowThreads), 0, stream,
+                         "combine_kernel", p);
+    });
+  });
+  DCOPY_API_END
+}
+
+int dcopy_expert_combine_grad(const DcopyMatrix *dy, const DcopyMatrix *dweights,
+                              const DcopyMatrix *dout, const DcopyMatrix *y, const int32_t *dest,
+                              int64_t slots, const int32_t *source, const DcopyMatrix *weights,
+                              dcopy_stream_t stream) {
+  DCOPY_API_BEGIN
+  if (!dy || !dweights || !dout || !y || !weights)
+    return set_error(DCOPY_ERR_PARAM_INVALID, "expert_combine_grad: NULL matrix");
+  if (int rc = check_matrix(dy, "dy", is_float(dy->type))) return rc;
+  if (int rc = check_matrix(dout, "dout", is_float(dout->type))) return rc;
+  if (int rc = check_matrix(y, "y", is_float(y->type))) return rc;
+  if (int rc = check_matrix(dweights, "dweights", dweights->type == kF32)) return rc;
+  if (int rc = check_width(dy, dout, "expert_combine_grad")) return rc;
+  if (int rc = check_width(dy, y, "expert_combine_grad")) return rc;
+  if (int rc = check_route(dest, dout->rows, slots, source, dy->rows, weights,
+                           "expert_combine_grad"))
+    return rc;
+  if (dy->rows != y->rows || dweights->rows != dout->rows || dweights->cols != slots)
+    return set_error(DCOPY_ERR_SHAPE_INVALID,
+                     "expert_combine_grad: dy has %lld rows for %lld of y, dweights is %lld x %lld",
+                     (long long)dy->rows, (long long)y->rows, (long long)dweights->rows,
+                     (long long)dweights->cols);
+  if (int rc = check_apart(dy, y, "expert_combine_grad")) return rc;
+  if (int rc = check_apart(dy, dout, "expert_combine_grad")) return rc;
+  Route p{};
+  p.out = dy->data;
+  p.in = y->data;
+  p.dout = dout->data;
+  p.dweights = static_cast<float *>(dweights->data);
+  p.out_pitch = dy->pitch;
+  p.in_pitch = y->pitch;
+  p.dout_pitch = dout->pitch;
+  p.w_pitch = weights->pitch;
+  p.dw_pitch = dweights->pitch;
+  p.dest = dest;
+  p.source = source;
+  p.weights = static_cast<const float *>(weights->data);
+  p.tokens = (uint32_t)dout->rows;
+  p.slots = (uint32_t)slots;
+  p.rows = (uint32_t)dy->rows;
+  p.token_blocks = p.tokens;
+  const uint32_t blocks = p.tokens + unused_blocks(source, dy->rows);
+  if (blocks == 0) return DCOPY_OK;
+  return with_float(dy->type, [&](auto t) {
+    using T = typename decltype(t)::type;
+    const int v = std::min(std::min(vector_width(dy), vector_width(dout)), vector_width(y));
+    return with_vector(v, [&](auto vw) {
+      constexpr int V = decltype(vw)::value;
+      p.vectors = (uint32_t)(dy->cols / V);
+      return launch_grid(combine_grad_kernel<T, V>, dim3(blocks), dim3(kRowThreads), 0, stream,
+                         "combine_grad_kernel", p);
+    });
+  });
+  DCOPY_API_END
+}
+
+}  // extern "C"

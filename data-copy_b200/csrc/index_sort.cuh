@@ -1,0 +1,37 @@
+// Stable sort of entries by a small whole-number key (index_sort.cu): the tokens of
+// an embedding gradient by id, a router's choices by expert.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "common.cuh"
+
+namespace dcopy {
+
+// Where the keys come from: `rows` x `cols` ids, row-major with a pitch.  An entry's
+// key is id - first when that lies in [0, keys), else `keys` (it belongs nowhere).
+struct KeySource {
+  const void *ids;
+  int64_t pitch;   // elements between rows
+  int64_t first;
+  uint32_t keys;
+  uint32_t wide;   // ids are 64-bit
+  uint32_t n;      // rows * cols
+  FastDiv cols;
+};
+
+// Workspace bytes of sort_by_key for n entries and keys values.
+uint64_t sort_by_key_bytes(uint64_t n, uint64_t keys);
+// key_out[p], pos_out[p]: the p-th entry in key order, equal keys in entry order.
+// Both arrays (n values each) lie in the workspace.
+int sort_by_key(const KeySource &src, void *workspace, const uint32_t **key_out,
+                const uint32_t **pos_out, cudaStream_t s);
+
+// The router's form: at most kMaxExperts keys, offsets padded to `align`.
+constexpr uint32_t kMaxExperts = 1023;
+uint64_t sort_experts_bytes(uint64_t n, uint32_t experts);
+int sort_experts(const KeySource &src, uint32_t align, int32_t *dest, int32_t *source,
+                 uint32_t rows, int32_t *offsets, void *workspace, cudaStream_t s);
+
+}  // namespace dcopy

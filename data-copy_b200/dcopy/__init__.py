@@ -19,6 +19,7 @@ Names follow the reference's host interface:
     FRACTAL_NZ transfers (base/formats/format_transfers/format_transfer_fractal_nz.cc);
   * ``zz_shape`` / ``nd_to_zz`` / ``zz_to_nd`` -- the same for FRACTAL_ZZ
     (base/formats/format_transfers/format_transfer_fractal_zz.cc).
+The operators of language models (``model_ops``) take tensors and read shapes from them.
 """
 from __future__ import annotations
 
@@ -46,6 +47,10 @@ __all__ = [
     "ERR_FORMAT_INVALID", "ERR_CUDA", "ERR_TIMEOUT", "ERR_UNSUPPORTED", "ERR_FAILED",
     "fz_shape", "to_fractal_z", "from_fractal_z", "TRANSFER_FRACTAL_Z", "TRANSFER_FRACTAL_Z_TBE",
     "TRANSFER_FRACZ_NCHW", "TRANSFER_FRACZ_HWCN", "TRANSFER_FRACZ_NHWC", "format_with_sub",
+    "DcopyMatrix", "DcopyGrad", "DcopyGradList", "embedding_lookup", "embedding_grad",
+    "embedding_grad_workspace", "expert_rows", "expert_sort", "expert_sort_workspace",
+    "expert_dispatch", "expert_combine", "expert_combine_grad", "GradList", "grad_sum_squares",
+    "grad_clip", "clip_grad_norm",
 ]
 
 OK = 0
@@ -151,6 +156,24 @@ MEMCPY_KIND = {"HOST_TO_HOST": 0, "HOST_TO_DEVICE": 1, "DEVICE_TO_HOST": 2,
                "HOST_TO_DEVICE_EX": 6, "DEVICE_TO_HOST_EX": 7, "DEFAULT": 8}
 
 
+class DcopyMatrix(ctypes.Structure):
+    """rows x cols elements of a GE data type, rows `pitch` elements apart."""
+    _fields_ = [("data", ctypes.c_void_p), ("rows", ctypes.c_int64), ("cols", ctypes.c_int64),
+                ("pitch", ctypes.c_int64), ("type", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+class DcopyGrad(ctypes.Structure):
+    """One gradient of a list: count elements from src, clipped into dst."""
+    _fields_ = [("src", ctypes.c_void_p), ("dst", ctypes.c_void_p), ("count", ctypes.c_uint64),
+                ("src_type", ctypes.c_int32), ("dst_type", ctypes.c_int32)]
+
+
+class DcopyGradList(ctypes.Structure):
+    """A list of gradients as dcopy_grad_list_build lays it out."""
+    _fields_ = [("workspace", ctypes.c_void_p), ("entries", ctypes.c_uint32),
+                ("chunks", ctypes.c_uint32)]
+
+
 class DcopyDevCopy(ctypes.Structure):
     """One device's strided copy for dcopy_copy_ext_multi."""
     _fields_ = [("device", ctypes.c_int32), ("dst", ctypes.c_void_p), ("src", ctypes.c_void_p),
@@ -164,6 +187,8 @@ _lib = None
 _vp = ctypes.c_void_p
 _i64p = ctypes.POINTER(ctypes.c_int64)
 _u64p = ctypes.POINTER(ctypes.c_uint64)
+_mat = ctypes.POINTER(DcopyMatrix)
+_grads = ctypes.POINTER(DcopyGradList)
 _SIGNATURES = {
     "dcopy_last_error_message": (ctypes.c_char_p, []),
     "dcopy_status_to_ge": (ctypes.c_uint32, [ctypes.c_int]),
@@ -254,6 +279,24 @@ _SIGNATURES = {
                                              ctypes.c_void_p]),
     "dcopy_memcpy_async_batch": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_uint32, ctypes.c_int32,
                                                 ctypes.c_void_p]),
+    "dcopy_embedding_lookup": (ctypes.c_int, [_mat, _mat, _mat, ctypes.c_int64, ctypes.c_float,
+                                              _vp]),
+    "dcopy_embedding_grad_workspace": (ctypes.c_int, [ctypes.c_int64] * 3 + [_u64p]),
+    "dcopy_embedding_grad": (ctypes.c_int, [_mat, _mat, _mat, ctypes.c_int64, ctypes.c_float,
+                                            ctypes.c_int32, _vp, ctypes.c_uint64, _vp]),
+    "dcopy_expert_rows": (ctypes.c_int, [ctypes.c_int64, ctypes.c_int32, ctypes.c_int32, _i64p]),
+    "dcopy_expert_sort_workspace": (ctypes.c_int, [ctypes.c_int64, ctypes.c_int32, _u64p]),
+    "dcopy_expert_sort": (ctypes.c_int, [_vp, _vp, ctypes.c_int64, _vp, _mat, ctypes.c_int32,
+                                         ctypes.c_int32, _vp, ctypes.c_uint64, _vp]),
+    "dcopy_expert_dispatch": (ctypes.c_int, [_mat, _mat, _vp, ctypes.c_int64, _vp, _mat, _vp]),
+    "dcopy_expert_combine": (ctypes.c_int, [_mat, _mat, _vp, ctypes.c_int64, _mat, _vp]),
+    "dcopy_expert_combine_grad": (ctypes.c_int, [_mat] * 4 + [_vp, ctypes.c_int64, _vp, _mat, _vp]),
+    "dcopy_grad_list_workspace": (ctypes.c_int, [ctypes.c_uint32, _u64p]),
+    "dcopy_grad_list_build": (ctypes.c_int, [_grads, ctypes.POINTER(DcopyGrad), ctypes.c_uint32,
+                                             _vp, ctypes.c_uint64, _vp]),
+    "dcopy_grad_sum_squares": (ctypes.c_int, [_grads, _vp, _vp]),
+    "dcopy_grad_clip": (ctypes.c_int, [_grads, _vp, ctypes.c_float, ctypes.c_float, _vp, _vp]),
+    "dcopy_clip_grad_norm": (ctypes.c_int, [_grads, ctypes.c_float, ctypes.c_float, _vp, _vp]),
 }
 
 
@@ -781,3 +824,9 @@ def memcpy_async(dst, dst_max: int, src, count: int, kind, stream=None) -> None:
     info = DcopyMemcpyInfo(addr(dst), dst_max, addr(src), count)
     _check(lib().dcopy_memcpy_async(ctypes.byref(info), kind, _stream(stream)),
            "dcopy_memcpy_async")
+
+
+from .model_ops import (GradList, clip_grad_norm, embedding_grad,  # noqa: E402
+                        embedding_grad_workspace, embedding_lookup, expert_combine,
+                        expert_combine_grad, expert_dispatch, expert_rows, expert_sort,
+                        expert_sort_workspace, grad_clip, grad_sum_squares)

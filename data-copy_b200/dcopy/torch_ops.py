@@ -20,6 +20,17 @@ as operators in the ``dcopy`` namespace, on CUDA tensors:
   torch.ops.dcopy.to_fractal_z(w, src_format, c0)     NCHW / NHWC / HWCN / ND weight -> FRACTAL_Z
   torch.ops.dcopy.from_fractal_z(w_fz, dst_format, dst_shape, c0)
                                                       FRACTAL_Z -> NCHW / NHWC / HWCN
+  torch.ops.dcopy.embedding(table, ids, scale, first_id)
+                                                      rows of a table by token id
+  torch.ops.dcopy.expert_sort(expert_ids, experts, align)
+                                                      (dest, source, offsets) of a router's choices
+  torch.ops.dcopy.expert_dispatch(x, dest, source)    tokens to their experts' rows
+  torch.ops.dcopy.expert_combine(y, dest, source, weights)
+                                                      and back, weighted and summed
+
+The last four differentiate through embedding_backward and expert_combine_backward, which
+are operators too; the gradients are those of dcopy.embedding_grad, dcopy.expert_combine_grad
+and, for the moves, each other.
 
 Lengths and gaps of the DataCopyExt operators count ELEMENTS of the tensors'
 dtype (as DataCopyPadExtend's arguments do, datacopy.h:14-40).  Each operator
@@ -28,7 +39,7 @@ tracing without a GPU.  Every call runs on torch's current CUDA stream.
 """
 from __future__ import annotations
 
-from typing import List
+from typing import List, Optional
 
 import torch
 from torch.library import custom_op
@@ -234,3 +245,137 @@ def from_fractal_z(w: torch.Tensor, dst_format: str, dst_shape: List[int],
 @from_fractal_z.register_fake
 def _from_fractal_z_fake(w, dst_format, dst_shape, c0=16):
     return w.new_empty(list(dst_shape))
+
+
+# ---- operators of language models ------------------------------------------------------
+
+
+def _dense(t: torch.Tensor) -> torch.Tensor:
+    """A gradient as autograd hands it over may be expanded or transposed."""
+    return t.contiguous()
+
+
+@custom_op("dcopy::embedding", mutates_args=(), device_types="cuda")
+def embedding(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0,
+              first_id: int = 0) -> torch.Tensor:
+    out = table.new_empty(list(ids.shape) + [table.shape[1]])
+    dcopy.embedding_lookup(out.view(-1, table.shape[1]), table, ids.contiguous(), scale, first_id)
+    return out
+
+
+@embedding.register_fake
+def _embedding_fake(table, ids, scale=1.0, first_id=0):
+    return table.new_empty(list(ids.shape) + [table.shape[1]])
+
+
+@custom_op("dcopy::embedding_backward", mutates_args=(), device_types="cuda")
+def embedding_backward(dout: torch.Tensor, ids: torch.Tensor, vocab: int, scale: float = 1.0,
+                       first_id: int = 0) -> torch.Tensor:
+    width = dout.shape[-1]
+    grad = dout.new_empty(vocab, width)
+    dcopy.embedding_grad(grad, _dense(dout).view(-1, width), ids.contiguous(), scale, first_id)
+    return grad
+
+
+@embedding_backward.register_fake
+def _embedding_backward_fake(dout, ids, vocab, scale=1.0, first_id=0):
+    return dout.new_empty(vocab, dout.shape[-1])
+
+
+def _embedding_setup(ctx, inputs, output):
+    table, ctx.ids, ctx.scale, ctx.first_id = inputs
+    ctx.vocab = table.shape[0]
+
+
+def _embedding_grad(ctx, dout):
+    return embedding_backward(dout, ctx.ids, ctx.vocab, ctx.scale, ctx.first_id), None, None, None
+
+
+embedding.register_autograd(_embedding_grad, setup_context=_embedding_setup)
+
+
+@custom_op("dcopy::expert_sort", mutates_args=(), device_types="cuda")
+def expert_sort(expert_ids: torch.Tensor, experts: int,
+                align: int = 1) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    whole = dict(dtype=torch.int32, device=expert_ids.device)
+    dest = torch.empty(expert_ids.shape, **whole)
+    source = torch.empty(dcopy.expert_rows(expert_ids.numel(), experts, align), **whole)
+    offsets = torch.empty(experts + 1, **whole)
+    dcopy.expert_sort(dest, source, offsets, expert_ids.contiguous(), align)
+    return dest, source, offsets
+
+
+@expert_sort.register_fake
+def _expert_sort_fake(expert_ids, experts, align=1):
+    whole = dict(dtype=torch.int32)
+    return (expert_ids.new_empty(expert_ids.shape, **whole),
+            expert_ids.new_empty(dcopy.expert_rows(expert_ids.numel(), experts, align), **whole),
+            expert_ids.new_empty(experts + 1, **whole))
+
+
+@custom_op("dcopy::expert_dispatch", mutates_args=(), device_types="cuda")
+def expert_dispatch(x: torch.Tensor, dest: torch.Tensor, source: torch.Tensor) -> torch.Tensor:
+    out = x.new_empty(source.numel(), x.shape[1])
+    dcopy.expert_dispatch(out, _dense(x), dest, source)
+    return out
+
+
+@expert_dispatch.register_fake
+def _expert_dispatch_fake(x, dest, source):
+    return x.new_empty(source.numel(), x.shape[1])
+
+
+@custom_op("dcopy::expert_combine", mutates_args=(), device_types="cuda")
+def expert_combine(y: torch.Tensor, dest: torch.Tensor, source: torch.Tensor,
+                   weights: Optional[torch.Tensor] = None) -> torch.Tensor:
+    out = y.new_empty(dest.shape[0], y.shape[1])
+    dcopy.expert_combine(out, _dense(y), dest, None if weights is None else _dense(weights))
+    return out
+
+
+@expert_combine.register_fake
+def _expert_combine_fake(y, dest, source, weights=None):
+    return y.new_empty(dest.shape[0], y.shape[1])
+
+
+@custom_op("dcopy::expert_combine_backward", mutates_args=(), device_types="cuda")
+def expert_combine_backward(dout: torch.Tensor, y: torch.Tensor, dest: torch.Tensor,
+                            source: torch.Tensor,
+                            weights: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    dy = y.new_empty(y.shape)
+    dweights = weights.new_empty(weights.shape)
+    dcopy.expert_combine_grad(dy, dweights, _dense(dout), _dense(y), dest, _dense(weights), source)
+    return dy, dweights
+
+
+@expert_combine_backward.register_fake
+def _expert_combine_backward_fake(dout, y, dest, source, weights):
+    return y.new_empty(y.shape), weights.new_empty(weights.shape)
+
+
+def _dispatch_setup(ctx, inputs, output):
+    _, ctx.dest, ctx.source = inputs
+
+
+def _dispatch_grad(ctx, dout):
+    return expert_combine(dout, ctx.dest, ctx.source, None), None, None
+
+
+expert_dispatch.register_autograd(_dispatch_grad, setup_context=_dispatch_setup)
+
+
+def _combine_setup(ctx, inputs, output):
+    y, ctx.dest, ctx.source, weights = inputs
+    ctx.weighted = weights is not None
+    ctx.save_for_backward(*((y, weights) if ctx.weighted else ()))
+
+
+def _combine_grad(ctx, dout):
+    if not ctx.weighted:
+        return expert_dispatch(dout, ctx.dest, ctx.source), None, None, None
+    dy, dweights = expert_combine_backward(dout, ctx.saved_tensors[0], ctx.dest, ctx.source,
+                                           ctx.saved_tensors[1])
+    return dy, None, None, dweights
+
+
+expert_combine.register_autograd(_combine_grad, setup_context=_combine_setup)

@@ -505,6 +505,104 @@ int dcopy_memcpy_async(const DcopyMemcpyInfo *info, int32_t kind, dcopy_stream_t
 int dcopy_memcpy_async_batch(const DcopyMemcpyInfo *infos, uint32_t count, int32_t kind,
                              dcopy_stream_t stream);
 
+/* ---- rows by index: embedding, experts, gradients -------------------------------
+ * Operators of language models that move or sum rows picked by index.  The
+ * reference has no counterpart.  Elements are FLOAT (0), FLOAT16 (1) or BF16 (27);
+ * sums are held in fp32 and rounded once, to nearest even.  Every result is the
+ * same on every run: no sum depends on the order in which blocks execute. */
+
+/* rows x cols elements of a GE DataType, rows `pitch` elements apart (at least
+ * cols; not looked at when rows <= 1).  data is aligned to the element. */
+typedef struct DcopyMatrix {
+  void *data;
+  int64_t rows, cols, pitch;
+  int32_t type;
+  int32_t reserved;
+} DcopyMatrix;
+
+/* out[i,:] = round(scale * table[id_i - first_id, :]), zero where id_i - first_id
+ * lies outside the table (a padding id, or another rank's part of a vocabulary that
+ * is split by rows).  ids: INT32 (3) or INT64 (9), read row by row; out has a row
+ * for each id.  out and table may differ in type.  out overlaps neither input. */
+int dcopy_embedding_lookup(const DcopyMatrix *out, const DcopyMatrix *table,
+                           const DcopyMatrix *ids, int64_t first_id, float scale,
+                           dcopy_stream_t stream);
+
+/* The lookup's gradient: grad[v,:] = round(scale * sum of dout[i,:] over the i with
+ * id_i - first_id == v), rows without such an i zeroed; with accumulate != 0 the sum
+ * is added to what grad holds (in fp32, rounded once) and other rows stay as they
+ * are.  The workspace (device memory) holds the sorted ids and partial sums. */
+int dcopy_embedding_grad_workspace(int64_t tokens, int64_t vocab, int64_t width,
+                                   uint64_t *bytes);
+int dcopy_embedding_grad(const DcopyMatrix *grad, const DcopyMatrix *dout, const DcopyMatrix *ids,
+                         int64_t first_id, float scale, int32_t accumulate, void *workspace,
+                         uint64_t workspace_bytes, dcopy_stream_t stream);
+
+/* Tokens sorted by expert.  expert_ids holds a router's choices, a row of slots for
+ * each token (INT32 or INT64); an id outside [0, experts) belongs to no expert (a
+ * dropped choice).  Entry e = token * slots + slot goes to row dest[e], -1 if it has
+ * no expert; the rows of expert x are [offsets[x], offsets[x+1]), its entries first
+ * and in entry order, offsets[x+1] - offsets[x] rounded up to a multiple of `align`.
+ * source[row] is the entry of a row, -1 where a row holds none.  rows, the length of
+ * source, is at least dcopy_expert_rows; experts is at most 1023. */
+int dcopy_expert_rows(int64_t entries, int32_t experts, int32_t align, int64_t *rows);
+int dcopy_expert_sort_workspace(int64_t entries, int32_t experts, uint64_t *bytes);
+int dcopy_expert_sort(int32_t *dest, int32_t *source, int64_t rows, int32_t *offsets,
+                      const DcopyMatrix *expert_ids, int32_t experts, int32_t align,
+                      void *workspace, uint64_t workspace_bytes, dcopy_stream_t stream);
+
+/* out[dest[i,j],:] = x[i,:], or round(weights[i,j] * x[i,:]); entries whose dest lies
+ * outside out's rows are skipped.  With source (out->rows values) the rows that hold
+ * no entry are zeroed, with NULL they stay as they are.  Without weights the rows are
+ * moved bit for bit, and INT8 (2) and UINT8 (4) are taken too.  weights: FLOAT,
+ * tokens x slots.  Also the gradient of dcopy_expert_combine without weights. */
+int dcopy_expert_dispatch(const DcopyMatrix *out, const DcopyMatrix *x, const int32_t *dest,
+                          int64_t slots, const int32_t *source, const DcopyMatrix *weights,
+                          dcopy_stream_t stream);
+/* out[i,:] = round(sum over j, ascending, of (weights[i,j] *) y[dest[i,j],:]); entries
+ * whose dest lies outside y's rows add nothing, whatever their weight.  weights NULL:
+ * the plain sum, which is the gradient of dcopy_expert_dispatch. */
+int dcopy_expert_combine(const DcopyMatrix *out, const DcopyMatrix *y, const int32_t *dest,
+                         int64_t slots, const DcopyMatrix *weights, dcopy_stream_t stream);
+/* The gradient of dcopy_expert_combine: dy[dest[i,j],:] = round(weights[i,j] * dout[i,:])
+ * and dweights[i,j] = sum of dout[i,:] * y[dest[i,j],:] (FLOAT; 0 for skipped entries).
+ * source as in dcopy_expert_dispatch, for the rows of dy. */
+int dcopy_expert_combine_grad(const DcopyMatrix *dy, const DcopyMatrix *dweights,
+                              const DcopyMatrix *dout, const DcopyMatrix *y, const int32_t *dest,
+                              int64_t slots, const int32_t *source, const DcopyMatrix *weights,
+                              dcopy_stream_t stream);
+
+/* One gradient of a list: count elements from src, clipped into dst (src itself for
+ * in place, else apart from it). */
+typedef struct DcopyGrad {
+  const void *src;
+  void *dst;
+  uint64_t count;
+  int32_t src_type, dst_type;
+} DcopyGrad;
+/* A list of gradients laid out for the kernels.  The caller keeps this record, the
+ * workspace (device memory, 16-byte aligned) and the gradients' buffers alive while
+ * it uses the list; calls on one list follow one another (one stream, or ordered).
+ * build checks every buffer, writes the workspace and synchronises `stream`. */
+typedef struct DcopyGradList {
+  void *workspace;
+  uint32_t entries, chunks;
+} DcopyGradList;
+int dcopy_grad_list_workspace(uint32_t n, uint64_t *bytes);
+int dcopy_grad_list_build(DcopyGradList *list, const DcopyGrad *grads, uint32_t n,
+                          void *workspace, uint64_t workspace_bytes, dcopy_stream_t stream);
+/* total[0] (device, fp64) = the sum of squares over the whole list. */
+int dcopy_grad_sum_squares(const DcopyGradList *list, double *total, dcopy_stream_t stream);
+/* norm = sqrt(total[0]); dst = round(c * src) with c = min(1, max_norm / (norm + eps)).
+ * norm (device, fp32; NULL: not written) gets the norm.  A rank that holds a part of
+ * the gradients adds up the totals of all ranks between the two calls.  A norm that is
+ * infinite or NaN goes into c as the formula has it. */
+int dcopy_grad_clip(const DcopyGradList *list, const double *total, float max_norm, float eps,
+                    float *norm, dcopy_stream_t stream);
+/* Both in turn, for gradients that are all here. */
+int dcopy_clip_grad_norm(const DcopyGradList *list, float max_norm, float eps, float *norm,
+                         dcopy_stream_t stream);
+
 /* ---- multi-GPU ----------------------------------------------------------------
  * No counterpart in the reference (its kernels run on one device).
  * Copies shard by splitting the blockCount range over devices with no

@@ -1,0 +1,125 @@
+"""Host-side checks of the operators of language models: sizes, layouts and refusals that are
+decided before any device work."""
+import ctypes
+
+import pytest
+import torch
+
+
+def _mat(dcopy, data=0x10000, rows=4, cols=8, pitch=8, code=0):
+    return ctypes.byref(dcopy.DcopyMatrix(data, rows, cols, pitch, code, 0))
+
+
+def test_expert_rows(dcopy):
+    assert dcopy.expert_rows(100, 8, 1) == 100
+    assert dcopy.expert_rows(100, 8, 16) == 220
+    assert dcopy.expert_rows(3, 8, 16) == 48  # at most 3 experts hold anything
+    assert dcopy.expert_rows(0, 8, 16) == 0
+    for args, code in (((-1, 8, 1), dcopy.ERR_PARAM_INVALID), ((1, 0, 1), dcopy.ERR_PARAM_INVALID),
+                       ((1, 8, 0), dcopy.ERR_PARAM_INVALID),
+                       ((1 << 31, 8, 1), dcopy.ERR_SHAPE_INVALID),
+                       (((1 << 31) - 1, 8, 2), dcopy.ERR_SHAPE_INVALID)):
+        with pytest.raises(dcopy.DcopyError) as e:
+            dcopy.expert_rows(*args)
+        assert e.value.code == code
+
+
+def test_workspaces_grow_with_their_arguments(dcopy):
+    a, b = dcopy.embedding_grad_workspace(1000, 50, 64), dcopy.embedding_grad_workspace(2000, 50, 64)
+    assert 0 < a < b
+    assert dcopy.expert_sort_workspace(1 << 20, 64) > dcopy.expert_sort_workspace(1 << 10, 64) > 0
+    for f, args in ((dcopy.embedding_grad_workspace, (-1, 5, 5)),
+                    (dcopy.embedding_grad_workspace, (1, 1 << 31, 5)),
+                    (dcopy.expert_sort_workspace, (5, 0))):
+        with pytest.raises(dcopy.DcopyError) as e:
+            f(*args)
+        assert e.value.code == dcopy.ERR_PARAM_INVALID
+    with pytest.raises(dcopy.DcopyError) as e:
+        dcopy.expert_sort_workspace(5, 1024)
+    assert e.value.code == dcopy.ERR_UNSUPPORTED
+
+
+@pytest.mark.parametrize("change,code", [
+    (dict(code=11), "ERR_DATATYPE_INVALID"), (dict(rows=-1), "ERR_SHAPE_INVALID"),
+    (dict(cols=1 << 31), "ERR_SHAPE_INVALID"), (dict(pitch=7), "ERR_PARAM_INVALID"),
+    (dict(data=0x10002), "ERR_PARAM_INVALID"), (dict(data=None), "ERR_PARAM_INVALID"),
+    (dict(pitch=1 << 62), "ERR_PARAM_INVALID"),
+])
+def test_matrix_checks(dcopy, change, code):
+    """Each bad field of a matrix is refused with its status."""
+    lib = dcopy.lib()
+    ids = _mat(dcopy, 0x40000, 4, 1, 1, 9)
+    rc = lib.dcopy_embedding_lookup(_mat(dcopy, **change), _mat(dcopy), ids, 0, 1.0, None)
+    assert rc == getattr(dcopy, code), lib.dcopy_last_error_message()
+
+
+def test_null_arguments(dcopy):
+    lib, m = dcopy.lib(), _mat(dcopy)
+    assert lib.dcopy_embedding_lookup(None, m, m, 0, 1.0, None) == dcopy.ERR_PARAM_INVALID
+    assert lib.dcopy_embedding_grad(m, None, m, 0, 1.0, 0, None, 0, None) == dcopy.ERR_PARAM_INVALID
+    assert lib.dcopy_expert_sort(None, None, 0, None, None, 4, 1, None, 0, None) == dcopy.ERR_PARAM_INVALID
+    assert lib.dcopy_expert_dispatch(m, None, None, 1, None, None, None) == dcopy.ERR_PARAM_INVALID
+    assert lib.dcopy_expert_combine(None, m, None, 1, None, None) == dcopy.ERR_PARAM_INVALID
+    assert lib.dcopy_expert_combine_grad(m, m, m, m, None, 1, None, None, None) == dcopy.ERR_PARAM_INVALID
+    assert lib.dcopy_grad_list_build(None, None, 0, None, 0, None) == dcopy.ERR_PARAM_INVALID
+    assert lib.dcopy_clip_grad_norm(None, 1.0, 1e-6, None, None) == dcopy.ERR_PARAM_INVALID
+    empty = dcopy.DcopyGradList()
+    assert lib.dcopy_grad_sum_squares(ctypes.byref(empty), None, None) == dcopy.ERR_PARAM_INVALID
+    for bound in (float("nan"), -1.0):
+        assert lib.dcopy_clip_grad_norm(ctypes.byref(empty), bound, 0.0, None, None) == \
+            dcopy.ERR_PARAM_INVALID
+
+
+def test_python_refuses_host_tensors(dcopy):
+    x, ids = torch.zeros(4, 8), torch.zeros(4, dtype=torch.int64)
+    with pytest.raises(ValueError):
+        dcopy.embedding_lookup(x, x, ids)
+    with pytest.raises(ValueError):
+        dcopy.expert_dispatch(x, x, ids)
+    with pytest.raises(ValueError):
+        dcopy.GradList([x])
+    with pytest.raises(ValueError):
+        dcopy.GradList([])
+
+
+def test_matrix_of_a_tensor(dcopy, monkeypatch):
+    """Rows and pitch that the binding reads from a tensor's shape and strides."""
+    from dcopy import model_ops
+
+    class Fake:  # a tensor's layout as if it lay in device memory
+        is_cuda = True
+
+        def __init__(self, t):
+            self.t = t
+
+        def __getattr__(self, name):
+            return getattr(self.t, name)
+
+    def read(t):
+        m = model_ops._matrix(Fake(t), "t")
+        return m.rows, m.cols, m.pitch, m.type
+
+    x = torch.zeros(6, 10, 16)
+    assert read(x) == (60, 16, 16, 0)
+    assert read(x[:, :, :8]) == (60, 8, 16, 0)
+    assert read(x[:, 3]) == (6, 16, 160, 0)
+    assert read(x[0]) == (10, 16, 16, 0)
+    assert read(x[2:3, 4:5]) == (1, 16, 16, 0)
+    assert read(torch.zeros(1, 5, 1, 7, dtype=torch.bfloat16)) == (5, 7, 7, 27)
+    assert read(torch.zeros(12, dtype=torch.int64)) == (1, 12, 0, 9)
+    assert read(torch.zeros(12, dtype=torch.int32)[::3]) == (4, 1, 3, 3)
+    assert read(torch.zeros(9, 1)) == (9, 1, 1, 0)
+    with pytest.raises(ValueError):
+        read(x[:, :5])  # two row pitches
+    with pytest.raises(ValueError):
+        read(torch.zeros(4, 6).t())  # columns that are not dense
+
+
+def test_records_match_the_c_abi(dcopy, tmp_path, monkeypatch):
+    import test_abi_layout as layout
+    monkeypatch.setattr(layout, "STRUCTS", {
+        "DcopyMatrix": ["data", "rows", "cols", "pitch", "type", "reserved"],
+        "DcopyGrad": ["src", "dst", "count", "src_type", "dst_type"],
+        "DcopyGradList": ["workspace", "entries", "chunks"],
+    })
+    layout.test_ctypes_records_match_the_c_abi(dcopy, tmp_path)
