@@ -19,80 +19,83 @@
 namespace dcopy {
 namespace {
 
-constexpr int kThreads = 512;
-constexpr int kV = 8;                         // elements a thread takes at once
-constexpr int kUnroll = 4;
-constexpr uint32_t kChunk = kThreads * kV * kUnroll;  // elements of one step of a block
+constexpr int kThreads = 256;
+constexpr int kUnroll = 4;  // 16-byte loads a thread has in flight
 
-// One tensor of the list as the kernels read it.
-struct Entry {
+// Elements of a chunk: large lists take 8192 (32 squares a thread in fp32, 0.2 % of
+// the bytes for the table of chunks); lists of fewer than kSmallList elements take
+// 2048, so that they still spread over all SMs (1.5 M fp32 elements: both passes
+// together 28.6 -> 9 us).
+constexpr uint32_t kChunk = 8192, kSmallChunk = 2048;
+constexpr uint64_t kSmallList = 8ull << 20;
+
+// A piece of one tensor.  `head` elements come before the first that starts a 16-byte
+// granule of src and a whole vector of dst; with head == count there is none.
+struct alignas(16) Chunk {
   const void *src;
   void *dst;
-  uint64_t count;
-  uint32_t first_chunk;  // chunks of the tensors before it
-  uint8_t src_type, dst_type, vector, pad;
+  uint32_t count, head;
+  uint64_t pad;
 };
-static_assert(sizeof(Entry) == 32, "Entry is 32 bytes");
+static_assert(sizeof(Chunk) == 32, "Chunk is 32 bytes");
 
-// The caller's buffer: a header, the entries, one partial sum a block.
-struct Header {
-  double total;
-  uint32_t done;   // blocks that have written their partial sum
-  uint32_t pad[13];
-};
-static_assert(sizeof(Header) == 64, "Header is 64 bytes");
-constexpr uint32_t kMaxBlocks = 4096;
+// The caller's buffer: one partial sum for each block of the first pass, the chunks,
+// those of one pair of types after the other (a kernel for each pair that occurs: one
+// kernel for all of them took 193 registers instead of 40).
+constexpr uint32_t kMaxBlocks = 2048;  // of one source type
+constexpr uint64_t kPartBytes = 3 * kMaxBlocks * sizeof(double);
+constexpr int kPairs = 9;
+constexpr int32_t kTypes[3] = {kF32, kF16, kBF16};
+
+int type_index(int32_t type) { return type == kF32 ? 0 : type == kF16 ? 1 : 2; }
 
 struct List {
-  Header *header;
-  const Entry *entry;
+  const Chunk *chunk;
   double *part;
-  uint32_t count, chunks;
+  uint32_t chunks;
 };
 
-// The entry that holds a chunk: the last whose first_chunk is not above it.
-__device__ __forceinline__ uint32_t find_entry(const List &l, uint32_t chunk) {
-  uint32_t lo = 0, hi = l.count - 1;
-  while (lo < hi) {
-    const uint32_t mid = (lo + hi + 1) / 2;
-    if (l.entry[mid].first_chunk <= chunk) lo = mid;
-    else hi = mid - 1;
-  }
-  return lo;
+__device__ __forceinline__ Chunk load_chunk(const Chunk *c) {
+  union {
+    Chunk chunk;
+    uint4 word[2];
+  } u;
+  u.word[0] = __ldg(reinterpret_cast<const uint4 *>(c));
+  u.word[1] = __ldg(reinterpret_cast<const uint4 *>(c) + 1);
+  return u.chunk;
 }
 
-// Calls f(vector, index of its first element) on this thread's vectors of one chunk,
-// kUnroll loads in flight.
-template <typename T, int V, typename F>
-__device__ __forceinline__ void each_vector(const T *src, uint64_t begin, uint64_t end, F &&f) {
-  constexpr int kSteps = kV / V * kUnroll;
+// Calls f(vector, first element) on this thread's share of a chunk: vectors of 16
+// bytes of src, U loads ahead, and single elements at the ends.  The share does not
+// depend on U.
+template <typename T, int U, typename F>
+__device__ __forceinline__ void each_vector(const Chunk &c, F &&f) {
+  constexpr uint32_t V = 16 / sizeof(T);
+  const T *src = static_cast<const T *>(c.src);
+  const uint32_t vectors = (c.count - c.head) / V, tail = c.head + vectors * V;
+#pragma unroll 1
+  for (uint32_t i0 = threadIdx.x; i0 < vectors; i0 += kThreads * U) {
+    Vec<T, V> in[U];
 #pragma unroll
-  for (int u0 = 0; u0 < kSteps; u0 += kUnroll) {
-    Vec<T, V> in[kUnroll];
+    for (int u = 0; u < U; ++u)
+      if (i0 + u * kThreads < vectors) in[u].load_plain(src + c.head + (i0 + u * kThreads) * V);
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const uint64_t e = begin + ((uint64_t)(u0 + u) * kThreads + threadIdx.x) * V;
-      if (e < end) in[u].load_plain(src + e);
-    }
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const uint64_t e = begin + ((uint64_t)(u0 + u) * kThreads + threadIdx.x) * V;
-      if (e < end) f(in[u], e);
-    }
+    for (int u = 0; u < U; ++u)
+      if (i0 + u * kThreads < vectors) f(in[u], c.head + (i0 + u * kThreads) * V);
   }
-}
-
-template <typename F>
-__device__ __forceinline__ void by_type(int type, F &&f) {
-  if (type == kF32) f(TypeTag<float>{});
-  else if (type == kF16) f(TypeTag<__half>{});
-  else f(TypeTag<__nv_bfloat16>{});
+  const uint32_t ends = c.head + c.count - tail;  // head and tail in one loop
+#pragma unroll 1
+  for (uint32_t i = threadIdx.x; i < ends; i += kThreads) {
+    const uint32_t e = i < c.head ? i : tail + i - c.head;
+    Vec<T, 1> in;
+    in.load_plain(src + e);
+    f(in, e);
+  }
 }
 
 __device__ __forceinline__ double block_sum(double v, double *warp_sum) {
 #pragma unroll
   for (int o = 16; o; o /= 2) v += __shfl_xor_sync(~0u, v, o);
-  __syncthreads();
   if (threadIdx.x % 32 == 0) warp_sum[threadIdx.x / 32] = v;
   __syncthreads();
   double all = 0.0;
@@ -101,162 +104,187 @@ __device__ __forceinline__ double block_sum(double v, double *warp_sum) {
   return all;
 }
 
-// This thread's sum of squares over one chunk: at most 32 of them, in fp32, unless
-// they leave fp32's range (above 2^128, or so small that what underflows could count):
-// then once more in fp64.
-template <typename T, int V>
-__device__ __forceinline__ double chunk_squares(const T *src, uint64_t begin, uint64_t end) {
+// This thread's sum of squares over one chunk in fp32, unless they leave its range
+// (above 2^127, or so small that what underflows could count): then again in fp64.
+template <typename T>
+__device__ __forceinline__ double chunk_squares(const Chunk &c) {
   float sum = 0.0f;
   uint32_t bits = 0;
-  each_vector<T, V>(src, begin, end, [&](const Vec<T, V> &v, uint64_t) {
+  each_vector<T, kUnroll>(c, [&](const auto &v, uint32_t) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) sum = fmaf(v.get(i), v.get(i), sum);
+    for (int i = 0; i < v.kSize; ++i) sum = fmaf(v.get(i), v.get(i), sum);
 #pragma unroll
-    for (int i = 0; i < Vec<T, V>::kWords; ++i) bits |= v.w[i];
+    for (int i = 0; i < v.kWords; ++i) bits |= v.w[i];
   });
   if (bits == 0 || (sum >= 0x1p-90f && sum < 0x1p+127f)) return sum;
   double wide = 0.0;
-  each_vector<T, V>(src, begin, end, [&](const Vec<T, V> &v, uint64_t) {
+  each_vector<T, 1>(c, [&](const auto &v, uint32_t) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) wide = fma((double)v.get(i), (double)v.get(i), wide);
+    for (int i = 0; i < v.kSize; ++i) wide = fma((double)v.get(i), (double)v.get(i), wide);
   });
   return wide;
 }
 
+template <typename T>
 __global__ void __launch_bounds__(kThreads) sum_squares_kernel(List l) {
   __shared__ double warp_sum[kThreads / 32];
-  __shared__ bool last;
   pdl_trigger_at_entry();
   pdl_wait();
   pdl_launch_dependents();
-  double wide = 0.0;
-  for (uint32_t chunk = blockIdx.x; chunk < l.chunks; chunk += gridDim.x) {
-    const Entry t = l.entry[find_entry(l, chunk)];
-    const uint64_t begin = (uint64_t)(chunk - t.first_chunk) * kChunk;
-    const uint64_t end = min(begin + kChunk, t.count);
-    by_type(t.src_type, [&](auto tag) {
-      using T = typename decltype(tag)::type;
-      const T *src = static_cast<const T *>(t.src);
-      wide += t.vector ? chunk_squares<T, kV>(src, begin, end)
-                       : chunk_squares<T, 1>(src, begin, end);
-    });
-  }
-  const double all = block_sum(wide, warp_sum);
-  if (threadIdx.x == 0) {
-    l.part[blockIdx.x] = all;
-    __threadfence();
-    last = atomicAdd(&l.header->done, 1u) == gridDim.x - 1;
-  }
-  __syncthreads();
-  if (!last) return;
-  __threadfence();
-  double v = 0.0;
-  for (uint32_t b = threadIdx.x; b < gridDim.x; b += kThreads) v += __ldcg(&l.part[b]);
-  v = block_sum(v, warp_sum);
-  if (threadIdx.x == 0) {
-    l.header->total = v;
-    l.header->done = 0;
-  }
-}
-
-__global__ void __launch_bounds__(kThreads) clip_kernel(List l, const double *total, float max_norm,
-                                                        float eps, float *norm_out) {
-  pdl_trigger_at_entry();
-  pdl_wait();
-  pdl_launch_dependents();
-  const float norm = (float)sqrt(*total);
-  const float ratio = max_norm / (norm + eps);
-  const float c = ratio < 1.0f || ratio != ratio ? ratio : 1.0f;  // NaN goes on
-  if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = norm;
+  double sum = 0.0;
+  Chunk next = load_chunk(l.chunk + blockIdx.x);
   for (uint32_t k = blockIdx.x; k < l.chunks; k += gridDim.x) {
-    const uint32_t chunk = l.chunks - 1 - k;  // what the first pass read last is still in L2
-    const Entry t = l.entry[find_entry(l, chunk)];
-    if (c == 1.0f && t.src == t.dst && t.src_type == t.dst_type) continue;  // nothing changes
-    const uint64_t begin = (uint64_t)(chunk - t.first_chunk) * kChunk;
-    const uint64_t end = min(begin + kChunk, t.count);
-    by_type(t.src_type, [&](auto tin) {
-      by_type(t.dst_type, [&](auto tout) {
-        using T = typename decltype(tin)::type;
-        using O = typename decltype(tout)::type;
-        const T *src = static_cast<const T *>(t.src);
-        O *dst = static_cast<O *>(t.dst);
-        auto write = [&](const auto &v, uint64_t e, auto width) {
-          constexpr int V = decltype(width)::value;
-          float f[V];
+    const Chunk c = next;
+    if (k + gridDim.x < l.chunks) next = load_chunk(l.chunk + k + gridDim.x);
+    sum += chunk_squares<T>(c);
+  }
+  sum = block_sum(sum, warp_sum);
+  if (threadIdx.x == 0) l.part[blockIdx.x] = sum;
+}
+
+// The sum of the first pass's partial sums, the same in every block.
+__device__ __forceinline__ double sum_parts(const double *part, uint32_t parts) {
+  __shared__ double warp_sum[kThreads / 32];
+  double v = 0.0;
+  for (uint32_t b = threadIdx.x; b < parts; b += kThreads) v += part[b];
+  return block_sum(v, warp_sum);
+}
+
+__global__ void __launch_bounds__(kThreads) total_kernel(List l, uint32_t parts, double *total) {
+  pdl_trigger_at_entry();
+  pdl_wait();
+  pdl_launch_dependents();
+  const double all = sum_parts(l.part, parts);
+  if (threadIdx.x == 0) *total = all;
+}
+
+// total NULL: the partial sums of the pass before are added up here, by every block.
+template <typename T, typename O>
+__global__ void __launch_bounds__(kThreads) clip_kernel(List l, uint32_t parts, const double *total,
+                                                        float max_norm, float eps, float *norm_out) {
+  pdl_trigger_at_entry();
+  pdl_wait();
+  pdl_launch_dependents();
+  const float norm = (float)sqrt(total ? *total : sum_parts(l.part, parts));
+  const float ratio = max_norm / (norm + eps);
+  const float f = ratio < 1.0f || ratio != ratio ? ratio : 1.0f;  // NaN goes on
+  if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = norm;
+  if (blockIdx.x >= l.chunks) return;
+  // Last chunk first: what the first pass read last is still in L2.
+  Chunk next = load_chunk(l.chunk + (l.chunks - 1 - blockIdx.x));
+  for (uint32_t k = blockIdx.x; k < l.chunks; k += gridDim.x) {
+    const Chunk c = next;
+    if (k + gridDim.x < l.chunks) next = load_chunk(l.chunk + (l.chunks - 1 - k - gridDim.x));
+    if (f == 1.0f && c.src == c.dst) continue;  // in place: nothing changes
+    O *dst = static_cast<O *>(c.dst);
+    each_vector<T, kUnroll>(c, [&](const auto &v, uint32_t e) {
+      constexpr int V = std::decay_t<decltype(v)>::kSize;
+      float g[V];
 #pragma unroll
-          for (int i = 0; i < V; ++i) f[i] = v.get(i) * c;
-          Vec<O, V> out;
-          out.put(f);
-          out.store(dst + e);
-        };
-        if (t.vector)
-          each_vector<T, kV>(src, begin, end, [&](const Vec<T, kV> &v, uint64_t e) {
-            write(v, e, std::integral_constant<int, kV>{});
-          });
-        else
-          each_vector<T, 1>(src, begin, end, [&](const Vec<T, 1> &v, uint64_t e) {
-            write(v, e, std::integral_constant<int, 1>{});
-          });
-      });
+      for (int i = 0; i < V; ++i) g[i] = v.get(i) * f;
+      Vec<O, V> out;
+      out.put(g);
+      out.store(dst + e);
     });
   }
 }
 
-// A tensor's elements that whole vectors cover, its two ends in a scalar entry each.
-struct Part {
-  uint64_t begin, count;
-  bool vector;
-};
-
-int split_tensor(const DcopyGrad &g, Part (&part)[3]) {
-  const int sb = elem_size(g.src_type), db = elem_size(g.dst_type);
+// Elements before the first at which src starts a 16-byte granule and dst a vector of
+// as many elements; count when there is none.
+uint64_t head_of(const DcopyGrad &g) {
+  const int sb = elem_size(g.src_type), db = elem_size(g.dst_type), v = 16 / sb;
   const uintptr_t s = (uintptr_t)g.src, d = (uintptr_t)g.dst;
-  // The first element at which both sides start a 16-byte granule, if there is one.
-  for (uint64_t head = 0; head < 8; ++head) {
-    if ((s + head * sb) % 16 || (d + head * db) % 16) continue;
-    if (g.count < head + kV) break;
-    const uint64_t body = (g.count - head) / kV * kV;
-    int n = 0;
-    if (head) part[n++] = {0, head, false};
-    part[n++] = {head, body, true};
-    if (head + body < g.count) part[n++] = {head + body, g.count - head - body, false};
-    return n;
-  }
-  part[0] = {0, g.count, false};
-  return g.count ? 1 : 0;
+  for (uint64_t head = 0; head < (uint64_t)v && head < g.count; ++head)
+    if ((s + head * sb) % 16 == 0 && (d + head * db) % std::min(16, v * db) == 0) return head;
+  return g.count;
 }
 
-uint64_t list_bytes(uint64_t n) {
-  return sizeof(Header) + kMaxBlocks * sizeof(double) + 3 * n * sizeof(Entry);
+// Chunks that grads can have at most, whatever their alignment: one more each than
+// their elements need, as heads shift the chunk ends.
+uint64_t most_chunks(const DcopyGrad *grads, uint32_t n, uint32_t size) {
+  uint64_t chunks = 0;
+  for (uint32_t i = 0; i < n; ++i) chunks += (grads[i].count + size - 1) / size + 1;
+  return chunks;
 }
 
-int open_list(const DcopyGradList *list, List *l) {
+uint32_t chunk_size(const DcopyGrad *grads, uint32_t n) {
+  uint64_t all = 0;
+  for (uint32_t i = 0; i < n; ++i) all += grads[i].count;
+  return all < kSmallList ? kSmallChunk : kChunk;
+}
+
+uint64_t list_bytes(uint64_t chunks) { return kPartBytes + chunks * sizeof(Chunk); }
+
+int check_grads(const DcopyGrad *grads, uint32_t n, const char *what) {
+  if (!grads && n) return set_error(DCOPY_ERR_PARAM_INVALID, "%s: NULL gradients", what);
+  if (n > (1u << 24)) return set_error(DCOPY_ERR_UNSUPPORTED, "%s: %u tensors", what, n);
+  for (uint32_t i = 0; i < n; ++i)
+    if (grads[i].count >> 40)
+      return set_error(DCOPY_ERR_SHAPE_INVALID, "%s: gradient %u has %llu elements", what, i,
+                       (unsigned long long)grads[i].count);
+  if (most_chunks(grads, n, chunk_size(grads, n)) >> 31)
+    return set_error(DCOPY_ERR_UNSUPPORTED, "%s: too many elements", what);
+  return DCOPY_OK;
+}
+
+int open_list(const DcopyGradList *list) {
   if (!list || !list->workspace)
     return set_error(DCOPY_ERR_PARAM_INVALID, "gradient list: not built");
+  return check_device_span(list->workspace, list_bytes(list->first[kPairs]), "workspace");
+}
+
+// The chunks [begin, end) of a list.
+List part_of(const DcopyGradList *list, uint32_t begin, uint32_t end) {
   uint8_t *w = static_cast<uint8_t *>(list->workspace);
-  l->header = reinterpret_cast<Header *>(w);
-  l->part = reinterpret_cast<double *>(w + sizeof(Header));
-  l->entry = reinterpret_cast<const Entry *>(w + sizeof(Header) + kMaxBlocks * sizeof(double));
-  l->count = list->entries;
-  l->chunks = list->chunks;
-  return check_device_span(w, sizeof(Header) + kMaxBlocks * sizeof(double) +
-                                  (uint64_t)list->entries * sizeof(Entry), "workspace");
+  return List{reinterpret_cast<const Chunk *>(w + kPartBytes) + begin,
+              reinterpret_cast<double *>(w), end - begin};
 }
 
 template <typename K>
-unsigned list_grid(K kernel, const List &l) {
-  return std::max(1u, std::min({l.chunks, resident_ctas(kernel, kThreads, 0), kMaxBlocks}));
+uint32_t list_grid(K kernel, uint32_t chunks) {
+  return std::min({chunks, resident_ctas(kernel, kThreads, 0), kMaxBlocks});
 }
 
-int run_sum(const List &l, cudaStream_t s) {
-  return launch(sum_squares_kernel, list_grid(sum_squares_kernel, l), dim3(kThreads), 0, s,
-                "sum_squares_kernel", l);
+// The first pass: a launch for each source type; *parts partial sums.
+int run_sum(const DcopyGradList *list, uint32_t *parts, cudaStream_t s) {
+  *parts = 0;
+  for (int t = 0; t < 3; ++t) {
+    const uint32_t begin = list->first[3 * t], end = list->first[3 * t + 3];
+    if (begin == end) continue;
+    List l = part_of(list, begin, end);
+    l.part += *parts;
+    const int rc = with_float(kTypes[t], [&](auto tag) {
+      auto k = sum_squares_kernel<typename decltype(tag)::type>;
+      const uint32_t grid = list_grid(k, l.chunks);
+      *parts += grid;
+      return launch(k, grid, dim3(kThreads), 0, s, "sum_squares_kernel", l);
+    });
+    if (rc) return rc;
+  }
+  return DCOPY_OK;
 }
 
-int run_clip(const List &l, const double *total, float max_norm, float eps, float *norm,
-             cudaStream_t s) {
-  return launch(clip_kernel, list_grid(clip_kernel, l), dim3(kThreads), 0, s, "clip_kernel", l,
-                total, max_norm, eps, norm);
+// The second: a launch for each pair of types, the last one first.  An empty list
+// still has a norm.
+int run_clip(const DcopyGradList *list, uint32_t parts, const double *total, float max_norm,
+             float eps, float *norm, cudaStream_t s) {
+  bool any = false;
+  for (int q = kPairs - 1; q >= 0; --q) {
+    const uint32_t begin = list->first[q], end = list->first[q + 1];
+    if (begin == end && (q > 0 || any)) continue;
+    any = true;
+    List l = part_of(list, begin, end);
+    l.part = part_of(list, 0, 0).part;
+    const int rc = with_float(kTypes[q / 3], [&](auto tin) {
+      return with_float(kTypes[q % 3], [&](auto tout) {
+        auto k = clip_kernel<typename decltype(tin)::type, typename decltype(tout)::type>;
+        return launch(k, std::max(1u, list_grid(k, l.chunks)), dim3(kThreads), 0, s, "clip_kernel",
+                      l, parts, total, max_norm, eps, norm);
+      });
+    });
+    if (rc) return rc;
+  }
+  return DCOPY_OK;
 }
 
 int check_bound(float max_norm, float eps, const char *what) {
@@ -272,10 +300,11 @@ using namespace dcopy;
 
 extern "C" {
 
-int dcopy_grad_list_workspace(uint32_t n, uint64_t *bytes) {
+int dcopy_grad_list_workspace(const DcopyGrad *grads, uint32_t n, uint64_t *bytes) {
   DCOPY_API_BEGIN
   if (!bytes) return set_error(DCOPY_ERR_PARAM_INVALID, "grad_list_workspace: NULL");
-  *bytes = list_bytes(n);
+  if (int rc = check_grads(grads, n, "grad_list_workspace")) return rc;
+  *bytes = list_bytes(most_chunks(grads, n, chunk_size(grads, n)));
   return DCOPY_OK;
   DCOPY_API_END
 }
@@ -283,72 +312,66 @@ int dcopy_grad_list_workspace(uint32_t n, uint64_t *bytes) {
 int dcopy_grad_list_build(DcopyGradList *list, const DcopyGrad *grads, uint32_t n,
                           void *workspace, uint64_t workspace_bytes, dcopy_stream_t stream) {
   DCOPY_API_BEGIN
-  if (!list || (!grads && n))
-    return set_error(DCOPY_ERR_PARAM_INVALID, "grad_list_build: NULL argument");
-  if (n > (1u << 24))
-    return set_error(DCOPY_ERR_UNSUPPORTED, "grad_list_build: %u tensors", n);
-  if (workspace_bytes < list_bytes(n) || (uintptr_t)workspace % 16)
+  if (!list) return set_error(DCOPY_ERR_PARAM_INVALID, "grad_list_build: NULL list");
+  if (int rc = check_grads(grads, n, "grad_list_build")) return rc;
+  const uint32_t size = chunk_size(grads, n);
+  const uint64_t need = list_bytes(most_chunks(grads, n, size));
+  if (workspace_bytes < need || (uintptr_t)workspace % 16)
     return set_error(DCOPY_ERR_PARAM_INVALID,
                      "grad_list_build: workspace of %llu bytes at %p, %llu needed, 16-byte aligned",
-                     (unsigned long long)workspace_bytes, workspace,
-                     (unsigned long long)list_bytes(n));
-  if (int rc = check_device_span(workspace, list_bytes(n), "workspace")) return rc;
-  std::vector<uint8_t> image(list_bytes(n));
-  Entry *entry = reinterpret_cast<Entry *>(image.data() + sizeof(Header) +
-                                           kMaxBlocks * sizeof(double));
-  uint32_t entries = 0;
-  uint64_t chunks = 0;
+                     (unsigned long long)workspace_bytes, workspace, (unsigned long long)need);
+  if (int rc = check_device_span(workspace, need, "workspace")) return rc;
+  std::vector<Chunk> chunks[kPairs];
   for (uint32_t i = 0; i < n; ++i) {
     const DcopyGrad &g = grads[i];
     if (!is_float(g.src_type) || !is_float(g.dst_type))
       return set_error(DCOPY_ERR_DATATYPE_INVALID, "gradient %u: element types %d and %d", i,
                        g.src_type, g.dst_type);
     if (g.count == 0) continue;
-    if (g.count >> 40)
-      return set_error(DCOPY_ERR_SHAPE_INVALID, "gradient %u: %llu elements", i,
-                       (unsigned long long)g.count);
     const uint64_t sb = elem_size(g.src_type), db = elem_size(g.dst_type);
     if ((uintptr_t)g.src % sb || (uintptr_t)g.dst % db)
       return set_error(DCOPY_ERR_PARAM_INVALID, "gradient %u is not aligned to its elements", i);
     if (int rc = check_device_span(g.src, g.count * sb, "gradient")) return rc;
     if (int rc = check_device_span(g.dst, g.count * db, "clipped gradient")) return rc;
-    if (g.src != g.dst || sb != db)  // in place, or apart
+    if (g.src != g.dst || g.src_type != g.dst_type)  // in place, or apart
       if (int rc = check_disjoint(g.src, g.count * sb, g.dst, g.count * db, "gradient")) return rc;
-    Part part[3];
-    const int parts = split_tensor(g, part);
-    for (int k = 0; k < parts; ++k) {
-      Entry &e = entry[entries++];
-      e.src = static_cast<const uint8_t *>(g.src) + part[k].begin * sb;
-      e.dst = static_cast<uint8_t *>(g.dst) + part[k].begin * db;
-      e.count = part[k].count;
-      e.first_chunk = (uint32_t)chunks;
-      e.src_type = (uint8_t)g.src_type;
-      e.dst_type = (uint8_t)g.dst_type;
-      e.vector = part[k].vector;
-      chunks += (part[k].count + kChunk - 1) / kChunk;
-      if (chunks >> 31)
-        return set_error(DCOPY_ERR_UNSUPPORTED, "grad_list_build: too many elements");
+    // The first chunk takes the head too; the others start on a vector.
+    const uint64_t head = head_of(g);
+    const bool scalar = head == g.count;
+    for (uint64_t at = 0; at < g.count;) {
+      const uint64_t most = at == 0 && !scalar ? head + size : size;
+      Chunk c{};
+      c.src = static_cast<const uint8_t *>(g.src) + at * sb;
+      c.dst = static_cast<uint8_t *>(g.dst) + at * db;
+      c.count = (uint32_t)std::min<uint64_t>(most, g.count - at);
+      c.head = scalar ? c.count : at == 0 ? (uint32_t)head : 0;
+      chunks[3 * type_index(g.src_type) + type_index(g.dst_type)].push_back(c);
+      at += c.count;
     }
   }
-  DCOPY_CUDA_TRY(cudaMemcpyAsync(workspace, image.data(), image.size(), cudaMemcpyHostToDevice,
-                                 stream));
-  DCOPY_CUDA_TRY(cudaStreamSynchronize(stream));
   list->workspace = workspace;
-  list->entries = entries;
-  list->chunks = (uint32_t)chunks;
+  list->first[0] = 0;
+  for (int q = 0; q < kPairs; ++q) {
+    const uint32_t begin = list->first[q];
+    list->first[q + 1] = begin + (uint32_t)chunks[q].size();
+    if (!chunks[q].empty())
+      DCOPY_CUDA_TRY(cudaMemcpyAsync(const_cast<Chunk *>(part_of(list, begin, begin).chunk),
+                                     chunks[q].data(), chunks[q].size() * sizeof(Chunk),
+                                     cudaMemcpyHostToDevice, stream));
+  }
+  DCOPY_CUDA_TRY(cudaStreamSynchronize(stream));
   return DCOPY_OK;
   DCOPY_API_END
 }
 
 int dcopy_grad_sum_squares(const DcopyGradList *list, double *total, dcopy_stream_t stream) {
   DCOPY_API_BEGIN
-  List l{};
-  if (int rc = open_list(list, &l)) return rc;
+  if (int rc = open_list(list)) return rc;
   if (int rc = check_device_span(total, sizeof(double), "total")) return rc;
-  if (int rc = run_sum(l, stream)) return rc;
-  DCOPY_CUDA_TRY(cudaMemcpyAsync(total, &l.header->total, sizeof(double), cudaMemcpyDeviceToDevice,
-                                 stream));
-  return DCOPY_OK;
+  uint32_t parts = 0;
+  if (int rc = run_sum(list, &parts, stream)) return rc;
+  return launch(total_kernel, 1, dim3(kThreads), 0, stream, "total_kernel", part_of(list, 0, 0),
+                parts, total);
   DCOPY_API_END
 }
 
@@ -356,12 +379,11 @@ int dcopy_grad_clip(const DcopyGradList *list, const double *total, float max_no
                     float *norm, dcopy_stream_t stream) {
   DCOPY_API_BEGIN
   if (int rc = check_bound(max_norm, eps, "grad_clip")) return rc;
-  List l{};
-  if (int rc = open_list(list, &l)) return rc;
+  if (int rc = open_list(list)) return rc;
   if (int rc = check_device_span(total, sizeof(double), "total")) return rc;
   if (norm)
     if (int rc = check_device_span(norm, sizeof(float), "norm")) return rc;
-  return run_clip(l, total, max_norm, eps, norm, stream);
+  return run_clip(list, 0, total, max_norm, eps, norm, stream);
   DCOPY_API_END
 }
 
@@ -369,12 +391,12 @@ int dcopy_clip_grad_norm(const DcopyGradList *list, float max_norm, float eps, f
                          dcopy_stream_t stream) {
   DCOPY_API_BEGIN
   if (int rc = check_bound(max_norm, eps, "clip_grad_norm")) return rc;
-  List l{};
-  if (int rc = open_list(list, &l)) return rc;
+  if (int rc = open_list(list)) return rc;
   if (norm)
     if (int rc = check_device_span(norm, sizeof(float), "norm")) return rc;
-  if (int rc = run_sum(l, stream)) return rc;
-  return run_clip(l, &l.header->total, max_norm, eps, norm, stream);
+  uint32_t parts = 0;
+  if (int rc = run_sum(list, &parts, stream)) return rc;
+  return run_clip(list, parts, nullptr, max_norm, eps, norm, stream);
   DCOPY_API_END
 }
 

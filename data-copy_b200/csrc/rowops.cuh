@@ -177,6 +177,7 @@ struct Words {
 // nothing; put() rounds each value once, to nearest even.
 template <typename T, int V>
 struct Vec : Words<(int)sizeof(T) * V> {
+  static constexpr int kSize = V;
   using Words<(int)sizeof(T) * V>::w;
   __device__ __forceinline__ float get(int i) const {
     if constexpr (sizeof(T) == 4) return Elem<T>::to(w[i]);

@@ -170,8 +170,7 @@ class DcopyGrad(ctypes.Structure):
 
 class DcopyGradList(ctypes.Structure):
     """A list of gradients as dcopy_grad_list_build lays it out."""
-    _fields_ = [("workspace", ctypes.c_void_p), ("entries", ctypes.c_uint32),
-                ("chunks", ctypes.c_uint32)]
+    _fields_ = [("workspace", ctypes.c_void_p), ("first", ctypes.c_uint32 * 10)]
 
 
 class DcopyDevCopy(ctypes.Structure):
@@ -291,7 +290,8 @@ _SIGNATURES = {
     "dcopy_expert_dispatch": (ctypes.c_int, [_mat, _mat, _vp, ctypes.c_int64, _vp, _mat, _vp]),
     "dcopy_expert_combine": (ctypes.c_int, [_mat, _mat, _vp, ctypes.c_int64, _mat, _vp]),
     "dcopy_expert_combine_grad": (ctypes.c_int, [_mat] * 4 + [_vp, ctypes.c_int64, _vp, _mat, _vp]),
-    "dcopy_grad_list_workspace": (ctypes.c_int, [ctypes.c_uint32, _u64p]),
+    "dcopy_grad_list_workspace": (ctypes.c_int, [ctypes.POINTER(DcopyGrad), ctypes.c_uint32,
+                                                 _u64p]),
     "dcopy_grad_list_build": (ctypes.c_int, [_grads, ctypes.POINTER(DcopyGrad), ctypes.c_uint32,
                                              _vp, ctypes.c_uint64, _vp]),
     "dcopy_grad_sum_squares": (ctypes.c_int, [_grads, _vp, _vp]),

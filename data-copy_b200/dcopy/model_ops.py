@@ -270,7 +270,8 @@ class GradList:
                 raise ValueError(f"gradient {k}: {g.numel()} elements for {o.numel()}")
             arr[k] = DcopyGrad(g.data_ptr(), o.data_ptr(), g.numel(), _code(g.dtype), _code(o.dtype))
         n = ctypes.c_uint64(0)
-        _check(lib().dcopy_grad_list_workspace(len(arr), ctypes.byref(n)), "dcopy_grad_list_workspace")
+        _check(lib().dcopy_grad_list_workspace(arr, len(arr), ctypes.byref(n)),
+               "dcopy_grad_list_workspace")
         self._anchor = self._grads[0]
         self._space = torch.empty(n.value, dtype=torch.uint8, device=self._anchor.device)
         self._list = DcopyGradList()

@@ -586,9 +586,9 @@ typedef struct DcopyGrad {
  * build checks every buffer, writes the workspace and synchronises `stream`. */
 typedef struct DcopyGradList {
   void *workspace;
-  uint32_t entries, chunks;
+  uint32_t first[10];  /* chunks of each pair of types: [first[k], first[k+1]) */
 } DcopyGradList;
-int dcopy_grad_list_workspace(uint32_t n, uint64_t *bytes);
+int dcopy_grad_list_workspace(const DcopyGrad *grads, uint32_t n, uint64_t *bytes);
 int dcopy_grad_list_build(DcopyGradList *list, const DcopyGrad *grads, uint32_t n,
                           void *workspace, uint64_t workspace_bytes, dcopy_stream_t stream);
 /* total[0] (device, fp64) = the sum of squares over the whole list. */

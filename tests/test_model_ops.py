@@ -120,6 +120,6 @@ def test_records_match_the_c_abi(dcopy, tmp_path, monkeypatch):
     monkeypatch.setattr(layout, "STRUCTS", {
         "DcopyMatrix": ["data", "rows", "cols", "pitch", "type", "reserved"],
         "DcopyGrad": ["src", "dst", "count", "src_type", "dst_type"],
-        "DcopyGradList": ["workspace", "entries", "chunks"],
+        "DcopyGradList": ["workspace", "first"],
     })
     layout.test_ctypes_records_match_the_c_abi(dcopy, tmp_path)
