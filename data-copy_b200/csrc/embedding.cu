@@ -63,13 +63,14 @@ __global__ void __launch_bounds__(kRowThreads) lookup_kernel(Lookup p) {
     for (int i = 0; i < V; ++i) f[i] = known ? in[u].get(i) * p.scale : 0.0f;
     Vec<TOut, V> out;
     out.put(f);
-    if (c < p.vectors) out.store(dst + (uint64_t)c * V);
+    if (c < p.vectors) out.store_cs(dst + (uint64_t)c * V);
   }
 }
 
 // ---- gradient -------------------------------------------------------------------
 
-constexpr uint32_t kPiece = 32;  // sorted entries that one block sums
+constexpr uint32_t kPiece = 32;      // sorted entries of a piece
+constexpr uint32_t kMaxPieces = 32;  // pieces of a block
 
 struct Grad {
   void *grad;
@@ -99,38 +100,47 @@ __device__ __forceinline__ void write_row(T *row, uint32_t c, const float (&sum)
 
 // One piece of the sorted list: runs of equal ids that lie inside it are summed and
 // written; what a run that crosses an end of the piece has here goes to head (it
-// began earlier) or tail (it begins here and goes on).
+// began earlier) or tail (it begins here and goes on).  Rows of kAhead tokens are
+// fetched before the first is added.
 template <typename TIn, typename TOut, int V, bool kAdd>
 __global__ void __launch_bounds__(kRowThreads) piece_sum_kernel(Grad p) {
+  // The ids of the block's pieces, one before and one behind; positions.
+  __shared__ uint32_t keys[kMaxPieces * kPiece + 2], places[kMaxPieces * kPiece];
   pdl_trigger_at_entry();
   pdl_wait();
   pdl_launch_dependents();
-  const uint32_t piece = blockIdx.x * (kRowThreads >> p.lx) + (threadIdx.x >> p.lx);
+  const uint32_t block_pieces = kRowThreads >> p.lx;
+  const uint32_t first = blockIdx.x * block_pieces * kPiece;  // entry
+  for (uint32_t i = threadIdx.x; i < block_pieces * kPiece + 2; i += kRowThreads) {
+    const uint32_t e = first + i;  // entry e - 1
+    keys[i] = e >= 1 && e <= p.n ? p.key[e - 1] : p.keys;
+    if (i >= 1 && i <= block_pieces * kPiece && e <= p.n) places[i - 1] = p.pos[e - 1];
+  }
+  __syncthreads();
+  const uint32_t local = (threadIdx.x >> p.lx) * kPiece, piece = first / kPiece + (threadIdx.x >> p.lx);
   const uint32_t c = (blockIdx.y << p.lx) + (threadIdx.x & ((1u << p.lx) - 1));
   if (piece >= p.pieces || c >= p.vectors) return;
-  const uint32_t b = piece * kPiece, e = min(b + kPiece, p.n);
+  const uint32_t count = min(kPiece, p.n - piece * kPiece);
   const TIn *dout = static_cast<const TIn *>(p.dout) + (uint64_t)c * V;
   TOut *grad = static_cast<TOut *>(p.grad);
-  uint32_t key = p.key[b];
-  bool open = b > 0 && p.key[b - 1] == key;  // the run began in an earlier piece
+  uint32_t key = keys[local + 1];
+  bool open = piece > 0 && keys[local] == key;  // the run began in an earlier piece
   float sum[V] = {};
-  constexpr int kAhead = 4;
-  for (uint32_t i0 = b; i0 < e && key < p.keys; i0 += kAhead) {
+  constexpr int kAhead = 8;
+  for (uint32_t i0 = 0; i0 < count && key < p.keys; i0 += kAhead) {
     Vec<TIn, V> in[kAhead];
-    uint32_t next[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+      if (i0 + j < count && keys[local + i0 + j + 1] < p.keys)
+        in[j].load(dout + (int64_t)places[local + i0 + j] * p.dout_pitch);
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
-      const uint32_t i = i0 + j;
-      if (i < e) in[j].load(dout + (int64_t)p.pos[i] * p.dout_pitch);
-      next[j] = i + 1 < p.n ? p.key[i + 1] : p.keys;
-    }
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
-      if (i0 + j >= e || key >= p.keys) break;
+      if (i0 + j >= count || key >= p.keys) break;
 #pragma unroll
       for (int v = 0; v < V; ++v) sum[v] += in[j].get(v);
-      if (next[j] != key || i0 + j + 1 == e) {
-        float *part = open ? p.head : next[j] == key ? p.tail : nullptr;
+      const uint32_t next = keys[local + i0 + j + 2];
+      if (next != key || i0 + j + 1 == count) {
+        float *part = open ? p.head : next == key ? p.tail : nullptr;
         if (part) {
           Vec<float, V> out;
           out.put(sum);
@@ -141,14 +151,14 @@ __global__ void __launch_bounds__(kRowThreads) piece_sum_kernel(Grad p) {
 #pragma unroll
         for (int v = 0; v < V; ++v) sum[v] = 0.0f;
         open = false;
-        key = next[j];
+        key = next;
       }
     }
   }
 }
 
 // The runs that begin in a piece and go on: tail of that piece plus the heads of the
-// following ones, in order.
+// following ones, in order, kAhead of them fetched before it is known how many count.
 template <typename TOut, int V, bool kAdd>
 __global__ void __launch_bounds__(kRowThreads) piece_join_kernel(Grad p) {
   pdl_trigger_at_entry();
@@ -167,45 +177,26 @@ __global__ void __launch_bounds__(kRowThreads) piece_join_kernel(Grad p) {
   part.load(p.tail + (uint64_t)piece * p.width + at);
 #pragma unroll
   for (int v = 0; v < V; ++v) sum[v] = part.get(v);
-  for (uint32_t q = piece + 1; q < p.pieces && p.key[q * kPiece] == key; ++q) {
-    part.load(p.head + (uint64_t)q * p.width + at);
+  constexpr int kAhead = 8;
+  bool on = true;
+  for (uint32_t q = piece + 1; on && q < p.pieces; q += kAhead) {
+    Vec<float, V> head[kAhead];
+    bool same[kAhead];
 #pragma unroll
-    for (int v = 0; v < V; ++v) sum[v] += part.get(v);
+    for (int j = 0; j < kAhead; ++j) {
+      same[j] = q + j < p.pieces && p.key[(q + j) * kPiece] == key;
+      if (q + j < p.pieces) head[j].load(p.head + (uint64_t)(q + j) * p.width + at);
+    }
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      on = on && same[j];
+      if (on) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) sum[v] += head[j].get(v);
+      }
+    }
   }
   write_row<TOut, V, kAdd>(static_cast<TOut *>(p.grad) + key * p.grad_pitch, c, sum, p.scale);
-}
-
-// Zeroes rows of `bytes` bytes, `pitch` bytes apart, in units of N bytes.
-template <int N>
-__global__ void __launch_bounds__(kRowThreads) zero_rows_kernel(uint8_t *dst, uint64_t pitch,
-                                                                uint64_t units, uint32_t rows) {
-  pdl_trigger_at_entry();
-  pdl_wait();
-  pdl_launch_dependents();
-  Words<N> z;
-  z.zero();
-  for (uint32_t r = blockIdx.y; r < rows; r += gridDim.y)
-    for (uint64_t c = (uint64_t)blockIdx.x * kRowThreads + threadIdx.x; c < units;
-         c += (uint64_t)gridDim.x * kRowThreads)
-      z.store(dst + r * pitch + c * N);
-}
-
-int zero_rows(const DcopyMatrix *m, cudaStream_t s) {
-  const int eb = elem_size(m->type);
-  uint64_t rows = m->rows, bytes = (uint64_t)m->cols * eb;
-  const uint64_t pitch = (uint64_t)m->pitch * eb;
-  if (rows <= 1 || pitch == bytes) bytes *= rows, rows = 1;
-  const uint64_t all = (uintptr_t)m->data | bytes | (rows > 1 ? pitch : 0);
-  const int unit = all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 2;
-  const uint64_t units = bytes / unit;
-  const uint64_t gy = std::min<uint64_t>(rows, 65535);
-  const uint64_t most = (uint64_t)sm_count() * 32;
-  const uint64_t gx = std::min<uint64_t>((units + kRowThreads - 1) / kRowThreads,
-                                         std::max<uint64_t>(1, most / gy));
-  auto k = unit == 16 ? zero_rows_kernel<16> : unit == 4 ? zero_rows_kernel<4> : zero_rows_kernel<2>;
-  return launch_grid(k, dim3((unsigned)gx, (unsigned)gy), dim3(kRowThreads), 0, s,
-                     "zero_rows_kernel", static_cast<uint8_t *>(m->data), pitch, units,
-                     (uint32_t)rows);
 }
 
 int id_source(const DcopyMatrix *ids, int64_t first, int64_t keys, KeySource *src) {
@@ -281,7 +272,7 @@ int dcopy_embedding_grad_workspace(int64_t tokens, int64_t vocab, int64_t width,
       width > kMaxWidth)
     return set_error(DCOPY_ERR_PARAM_INVALID, "embedding_grad_workspace: %lld tokens, %lld x %lld",
                      (long long)tokens, (long long)vocab, (long long)width);
-  const uint64_t sort = (sort_by_key_bytes(tokens, vocab) + 15) / 16 * 16;
+  const uint64_t sort = (sort_by_key_bytes(tokens) + 15) / 16 * 16;
   const uint64_t row = ((uint64_t)width * sizeof(float) + 15) / 16 * 16;
   *bytes = sort + 2 * pieces_of(tokens) * row + 32;
   return DCOPY_OK;
@@ -314,13 +305,20 @@ int dcopy_embedding_grad(const DcopyMatrix *grad, const DcopyMatrix *dout, const
   if (int rc = check_apart(grad, dout, "embedding_grad")) return rc;
   if (int rc = check_apart(grad, ids, "embedding_grad")) return rc;
   if (grad->rows == 0 || grad->cols == 0) return DCOPY_OK;
-  if (!accumulate)
-    if (int rc = zero_rows(grad, stream)) return rc;
-  if (src.n == 0) return DCOPY_OK;
+  Fill fill;
+  if (!accumulate) {
+    const uint64_t eb = elem_size(grad->type);
+    fill.dst = static_cast<uint8_t *>(grad->data);
+    fill.rows = grad->rows;
+    fill.bytes = grad->cols * eb;
+    fill.pitch = grad->pitch * eb;
+    if (fill.rows == 1 || fill.pitch == fill.bytes) fill.bytes *= fill.rows, fill.rows = 1;
+  }
+  if (src.n == 0) return fill_zero(fill, stream);
   uint8_t *ws = reinterpret_cast<uint8_t *>(((uintptr_t)workspace + 15) / 16 * 16);
-  const uint64_t sort = (sort_by_key_bytes(src.n, grad->rows) + 15) / 16 * 16;
+  const uint64_t sort = (sort_by_key_bytes(src.n) + 15) / 16 * 16;
   Grad p{};
-  if (int rc = sort_by_key(src, ws, &p.key, &p.pos, stream)) return rc;
+  if (int rc = sort_by_key(src, fill, ws, &p.key, &p.pos, stream)) return rc;
   p.grad = grad->data;
   p.dout = dout->data;
   p.grad_pitch = grad->pitch;
@@ -339,7 +337,7 @@ int dcopy_embedding_grad(const DcopyMatrix *grad, const DcopyMatrix *dout, const
       return with_vector(std::min(vector_width(dout), vector_width(grad)), [&](auto vw) {
         constexpr int V = decltype(vw)::value;
         p.vectors = (uint32_t)(grad->cols / V);
-        const RowSplit split = split_rows(p.pieces, p.vectors, 1);
+        const RowSplit split = split_rows(p.pieces, p.vectors, 1, kMaxPieces);
         p.lx = split.lx;
         auto sum = accumulate ? piece_sum_kernel<TIn, TOut, V, true>
                               : piece_sum_kernel<TIn, TOut, V, false>;

@@ -28,25 +28,33 @@ struct Route {
   int64_t out_pitch, in_pitch, dout_pitch, w_pitch, dw_pitch;
   const int32_t *dest, *source;
   const float *weights;
-  uint32_t tokens, slots, rows, vectors, token_blocks;
+  uint32_t tokens, slots, rows, vectors, unused_blocks;
   int lx;
 };
 
-// Rows of the buffer in expert order that hold no entry are zeroed: this part of
-// the grid looks at kRowThreads rows a block.
+// Rows of the buffer in expert order that hold no entry are zeroed by the first
+// blocks of the grid, kUnusedRows rows each: padding comes in runs of rows, and
+// ahead of the others these blocks do not trail the kernel.
+constexpr uint32_t kUnusedRows = 128;
+
 template <int N>
-__device__ __forceinline__ void zero_unused(const Route &p, uint32_t block, void *rows) {
-  const uint32_t lane = threadIdx.x & 31;
-  const uint32_t r = block * kRowThreads + threadIdx.x;
-  uint32_t empty = __ballot_sync(~0u, r < p.rows && p.source[r] < 0);
+__device__ __forceinline__ void zero_unused(const Route &p, uint64_t row_bytes) {
+  __shared__ uint32_t masks[kUnusedRows / 32];
+  const uint32_t r0 = blockIdx.x * kUnusedRows, r = r0 + threadIdx.x;
+  if (threadIdx.x < kUnusedRows) {
+    const uint32_t empty = __ballot_sync(~0u, r < p.rows && p.source[r] < 0);
+    if (threadIdx.x % 32 == 0) masks[threadIdx.x / 32] = empty;
+  }
+  __syncthreads();
   Words<N> z;
   z.zero();
-  for (; empty; empty &= empty - 1) {
-    const uint32_t row = (r & ~31u) + __ffs(empty) - 1;
-    uint8_t *at = static_cast<uint8_t *>(rows) + row * p.out_pitch;
-    for (uint32_t c = blockIdx.y * 32 + lane; c < p.vectors; c += gridDim.y * 32)
-      z.store(at + (uint64_t)c * N);
-  }
+  for (uint32_t m = 0; m < kUnusedRows / 32; ++m)
+    for (uint32_t empty = masks[m]; empty; empty &= empty - 1) {
+      uint8_t *row = static_cast<uint8_t *>(p.out) + (r0 + 32 * m + __ffs(empty) - 1) * row_bytes;
+      for (uint32_t c = blockIdx.y * kRowThreads + threadIdx.x; c < p.vectors;
+           c += gridDim.y * kRowThreads)
+        z.store_cs(row + (uint64_t)c * N);
+    }
 }
 
 // Rows moved as N-byte units; pitches in bytes.
@@ -55,8 +63,9 @@ __global__ void __launch_bounds__(kRowThreads) dispatch_kernel(Route p) {
   pdl_trigger_at_entry();
   pdl_wait();
   pdl_launch_dependents();
-  if (blockIdx.x >= p.token_blocks) return zero_unused<N>(p, blockIdx.x - p.token_blocks, p.out);
-  const uint32_t token = blockIdx.x * (kRowThreads >> p.lx) + (threadIdx.x >> p.lx);
+  if (blockIdx.x < p.unused_blocks) return zero_unused<N>(p, p.out_pitch);
+  const uint32_t token =
+      (blockIdx.x - p.unused_blocks) * (kRowThreads >> p.lx) + (threadIdx.x >> p.lx);
   if (token >= p.tokens) return;
   const uint32_t step = 1u << p.lx;
   const uint32_t c0 = (blockIdx.y * U << p.lx) + (threadIdx.x & (step - 1));
@@ -72,7 +81,7 @@ __global__ void __launch_bounds__(kRowThreads) dispatch_kernel(Route p) {
     uint8_t *dst = static_cast<uint8_t *>(p.out) + row * p.out_pitch;
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (c0 + u * step < p.vectors) in[u].store(dst + (uint64_t)(c0 + u * step) * N);
+      if (c0 + u * step < p.vectors) in[u].store_cs(dst + (uint64_t)(c0 + u * step) * N);
   }
 }
 
@@ -82,11 +91,10 @@ __global__ void __launch_bounds__(kRowThreads) dispatch_weighted_kernel(Route p)
   pdl_trigger_at_entry();
   pdl_wait();
   pdl_launch_dependents();
-  if (blockIdx.x >= p.token_blocks) {
-    p.out_pitch *= sizeof(T);
-    return zero_unused<(int)sizeof(T) * V>(p, blockIdx.x - p.token_blocks, p.out);
-  }
-  const uint32_t token = blockIdx.x * (kRowThreads >> p.lx) + (threadIdx.x >> p.lx);
+  if (blockIdx.x < p.unused_blocks)
+    return zero_unused<(int)sizeof(T) * V>(p, p.out_pitch * sizeof(T));
+  const uint32_t token =
+      (blockIdx.x - p.unused_blocks) * (kRowThreads >> p.lx) + (threadIdx.x >> p.lx);
   const uint32_t c = (blockIdx.y << p.lx) + (threadIdx.x & ((1u << p.lx) - 1));
   if (token >= p.tokens || c >= p.vectors) return;
   Vec<T, V> in;
@@ -139,7 +147,7 @@ __global__ void __launch_bounds__(kRowThreads) combine_kernel(Route p) {
   }
   Vec<T, V> out;
   out.put(sum);
-  out.store(static_cast<T *>(p.out) + token * p.out_pitch + (uint64_t)c * V);
+  out.store_cs(static_cast<T *>(p.out) + token * p.out_pitch + (uint64_t)c * V);
 }
 
 // A block takes a token: its dout row meets each of the token's rows of y.
@@ -149,11 +157,9 @@ __global__ void __launch_bounds__(kRowThreads) combine_grad_kernel(Route p) {
   pdl_trigger_at_entry();
   pdl_wait();
   pdl_launch_dependents();
-  if (blockIdx.x >= p.token_blocks) {
-    p.out_pitch *= sizeof(T);
-    return zero_unused<(int)sizeof(T) * V>(p, blockIdx.x - p.token_blocks, p.out);
-  }
-  const uint32_t token = blockIdx.x;
+  if (blockIdx.x < p.unused_blocks)
+    return zero_unused<(int)sizeof(T) * V>(p, p.out_pitch * sizeof(T));
+  const uint32_t token = blockIdx.x - p.unused_blocks;
   const T *dout = static_cast<const T *>(p.dout) + token * p.dout_pitch;
   for (uint32_t j = 0; j < p.slots; ++j) {
     const int32_t row = p.dest[(uint64_t)token * p.slots + j];
@@ -175,7 +181,7 @@ __global__ void __launch_bounds__(kRowThreads) combine_grad_kernel(Route p) {
           f[i] = d * w;
         }
         out.put(f);
-        out.store(dy + (uint64_t)c * V);
+        out.store_cs(dy + (uint64_t)c * V);
       }
     }
 #pragma unroll
@@ -224,7 +230,7 @@ int check_width(const DcopyMatrix *a, const DcopyMatrix *b, const char *what) {
 }
 
 uint32_t unused_blocks(const int32_t *source, uint64_t rows) {
-  return source ? (uint32_t)((rows + kRowThreads - 1) / kRowThreads) : 0;
+  return source ? (uint32_t)((rows + kUnusedRows - 1) / kUnusedRows) : 0;
 }
 
 }  // namespace
@@ -336,8 +342,8 @@ int dcopy_expert_dispatch(const DcopyMatrix *out, const DcopyMatrix *x, const in
         p.vectors = (uint32_t)(out->cols / V);
         RowSplit split = split_rows(p.tokens, p.vectors, 1);
         p.lx = split.lx;
-        p.token_blocks = split.grid.x;
-        split.grid.x += unused_blocks(source, out->rows);
+        p.unused_blocks = unused_blocks(source, out->rows);
+        split.grid.x += p.unused_blocks;
         if (split.grid.x == 0) return (int)DCOPY_OK;
         return launch_grid(dispatch_weighted_kernel<T, V>, split.grid, dim3(kRowThreads), 0, stream,
                            "dispatch_weighted_kernel", p);
@@ -354,8 +360,8 @@ int dcopy_expert_dispatch(const DcopyMatrix *out, const DcopyMatrix *x, const in
   p.vectors = (uint32_t)(bytes / unit);
   RowSplit split = split_rows(p.tokens, p.vectors, 1);
   p.lx = split.lx;
-  p.token_blocks = split.grid.x;
-  split.grid.x += unused_blocks(source, out->rows);
+  p.unused_blocks = unused_blocks(source, out->rows);
+  split.grid.x += p.unused_blocks;
   if (split.grid.x == 0) return DCOPY_OK;
   auto k = unit == 16 ? dispatch_kernel<16, 1> : unit == 8 ? dispatch_kernel<8, 1>
            : unit == 4 ? dispatch_kernel<4, 1> : unit == 2 ? dispatch_kernel<2, 1>
@@ -440,8 +446,8 @@ int dcopy_expert_combine_grad(const DcopyMatrix *dy, const DcopyMatrix *dweights
   p.tokens = (uint32_t)dout->rows;
   p.slots = (uint32_t)slots;
   p.rows = (uint32_t)dy->rows;
-  p.token_blocks = p.tokens;
-  const uint32_t blocks = p.tokens + unused_blocks(source, dy->rows);
+  p.unused_blocks = unused_blocks(source, dy->rows);
+  const uint32_t blocks = p.tokens + p.unused_blocks;
   if (blocks == 0) return DCOPY_OK;
   return with_float(dy->type, [&](auto t) {
     using T = typename decltype(t)::type;

@@ -1,12 +1,13 @@
 // Stable sort by a small whole-number key.
 //
-// Counting sort over digits of up to 10 bits, lowest first.  One pass: every
-// tile of kTile entries counts its digits (tile_count_kernel); then each tile
-// ranks its entries again and writes them behind the digits below its own, the
-// same digit's entries of earlier tiles, of earlier warps of the tile, and of
-// earlier entries of the warp (tile_place_kernel).  Nothing depends on the order
-// in which tiles or atomics run, so the result is the same every time.
-// Experts fit one digit; token ids take two up to 2^20 and three beyond.
+// Counting sort by digits, lowest first.  One pass: every tile
+// of entries counts its digits (tile_count_kernel); then each tile ranks its entries
+// again and writes them behind the digits below its own, the same digit's entries of
+// earlier tiles, of earlier warps of the tile, and of earlier entries of the warp
+// (tile_place_kernel).  Nothing depends on the order in which tiles or atomics run,
+// so the result is the same every time.  Experts fit one digit of up to 10 bits; token
+// ids take two of up to 9 bits below 2^18 and three below 2^27.  What fits one tile
+// takes one launch for all digits.
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -15,15 +16,16 @@
 #include "common.cuh"
 #include "index_sort.cuh"
 #include "launch.cuh"
+#include "rowops.cuh"
 
 namespace dcopy {
 namespace {
 
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
-constexpr int kItems = 8;
-constexpr uint32_t kTile = kThreads * kItems;
-constexpr uint32_t kMaxBins = 1024;
+constexpr int kExpertBits = 10, kTokenBits = 9;  // digits of the two sorts, at most
+constexpr uint32_t kMaxBins = 1 << kExpertBits;
+constexpr uint32_t kOneTile = 8 * kThreads;
 
 __device__ __forceinline__ uint32_t entry_key(const KeySource &k, uint32_t e) {
   const uint32_t r = k.cols.div(e);
@@ -39,8 +41,11 @@ struct Pass {
   const uint32_t *key_in;   // ... later ones the pairs of the pass before
   const uint32_t *pos_in;
   uint32_t *key_out, *pos_out;
-  uint32_t *counts;         // [tiles][bins]
+  uint32_t *counts;         // [bins][tiles]
   uint32_t n, tiles, bins, shift;
+  uint32_t passes, bits;    // of the sort in one tile
+  Fill fill;
+  uint32_t fill_share, fill_shares;
 };
 
 struct ExpertOut {
@@ -52,22 +57,34 @@ __device__ __forceinline__ uint32_t load_key(const Pass &p, uint32_t e) {
   return p.key_in ? p.key_in[e] : entry_key(p.src, e);
 }
 
-__global__ void __launch_bounds__(kThreads) tile_count_kernel(Pass p) {
-  __shared__ uint32_t count[kMaxBins];
-  pdl_trigger_at_entry();
-  for (uint32_t d = threadIdx.x; d < p.bins; d += kThreads) count[d] = 0;
-  __syncthreads();
-  pdl_wait();
-  pdl_launch_dependents();
-  const uint32_t e0 = blockIdx.x * kTile + threadIdx.x;
-#pragma unroll
-  for (int i = 0; i < kItems; ++i) {
-    const uint32_t e = e0 + i * kThreads;
-    if (e < p.n) atomicAdd(&count[(load_key(p, e) >> p.shift) & (kMaxBins - 1)], 1u);
+// Share `share` of `shares` of the memory to zero, by blocks `block` of `blocks`.
+__device__ __forceinline__ void zero_share(const Fill &f, uint32_t share, uint32_t shares,
+                                           uint32_t block, uint32_t blocks) {
+  const uint32_t head0 = (uint32_t)(-(uintptr_t)f.dst & 15);
+  if (f.rows <= 1) {
+    const uint64_t head = min((uint64_t)head0, f.bytes), units = (f.bytes - head) / 16;
+    uint4 *dst = reinterpret_cast<uint4 *>(f.dst + head);
+    const uint64_t end = units * (share + 1) / shares;
+    for (uint64_t u = units * share / shares + (uint64_t)block * kThreads + threadIdx.x; u < end;
+         u += (uint64_t)blocks * kThreads)
+      dst[u] = make_uint4(0, 0, 0, 0);
+    if (share == 0 && block == 0) {
+      const uint64_t tail = f.bytes - head - units * 16;
+      if (threadIdx.x < head) f.dst[threadIdx.x] = 0;
+      if (threadIdx.x < tail) f.dst[f.bytes - 1 - threadIdx.x] = 0;
+    }
+    return;
   }
-  __syncthreads();
-  for (uint32_t d = threadIdx.x; d < p.bins; d += kThreads)
-    p.counts[blockIdx.x * p.bins + d] = count[d];
+  const uint64_t end = f.rows * (share + 1) / shares;
+  for (uint64_t r = f.rows * share / shares + block; r < end; r += blocks) {
+    uint8_t *row = f.dst + r * f.pitch;
+    const uint64_t head = min((uint64_t)(-(uintptr_t)row & 15), f.bytes);
+    const uint64_t units = (f.bytes - head) / 16, tail = f.bytes - head - units * 16;
+    for (uint64_t u = threadIdx.x; u < units; u += kThreads)
+      reinterpret_cast<uint4 *>(row + head)[u] = make_uint4(0, 0, 0, 0);
+    if (threadIdx.x < head) row[threadIdx.x] = 0;
+    if (threadIdx.x < tail) row[f.bytes - 1 - threadIdx.x] = 0;
+  }
 }
 
 // Exclusive sum over the block of one value a thread; *total gets the sum.
@@ -94,65 +111,133 @@ __device__ __forceinline__ uint32_t block_exclusive(uint32_t v, uint32_t *warp_s
   return before + x - v;
 }
 
-template <bool kExperts>
+// Entries of each digit that a warp of the tile holds, then that earlier warps hold.
+template <uint32_t kBins>
+struct Seen {
+  uint16_t of[kWarps][kBins];
+};
+
+template <uint32_t kBins>
+__device__ __forceinline__ void clear_seen(Seen<kBins> &seen, uint32_t bins) {
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (uint32_t d = 2 * lane; d < bins; d += 64)
+    *reinterpret_cast<uint32_t *>(&seen.of[warp][d]) = 0;
+}
+
+// rank[i]: entries of the same digit that precede the thread's i-th entry in its
+// warp.  Warp w holds entries [w * 32 * kItems, ...) of the tile, lane by lane.
+template <int kItems, uint32_t kBins>
+__device__ __forceinline__ void rank_in_warp(Seen<kBins> &seen, const uint32_t (&digit)[kItems],
+                                             uint32_t first, uint32_t n,
+                                             uint32_t (&rank)[kItems]) {
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int i = 0; i < kItems; ++i) {
+    const bool in = first + i * 32 < n;
+    const uint32_t lanes = __ballot_sync(~0u, in);
+    rank[i] = 0;
+    if (in) {
+      const uint32_t same = __match_any_sync(lanes, digit[i]);
+      const uint32_t before = seen.of[warp][digit[i]];
+      __syncwarp(lanes);
+      rank[i] = before + __popc(same & ((1u << lane) - 1));
+      if ((same >> lane) == 1) seen.of[warp][digit[i]] = (uint16_t)(before + __popc(same));
+      __syncwarp(lanes);
+    }
+  }
+}
+
+// seen becomes the entries of earlier warps; returns those of the tile.
+template <uint32_t kBins>
+__device__ __forceinline__ uint32_t sum_over_warps(Seen<kBins> &seen, uint32_t d) {
+  uint32_t run = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    const uint32_t c = seen.of[w][d];
+    seen.of[w][d] = (uint16_t)run;
+    run += c;
+  }
+  return run;
+}
+
+template <int kItems>
+__global__ void __launch_bounds__(kThreads) tile_count_kernel(Pass p) {
+  __shared__ uint32_t count[kMaxBins];
+  pdl_trigger_at_entry();
+  for (uint32_t d = threadIdx.x; d < p.bins; d += kThreads) count[d] = 0;
+  __syncthreads();
+  pdl_wait();
+  pdl_launch_dependents();
+  if (blockIdx.x >= p.tiles)
+    return zero_share(p.fill, p.fill_share, p.fill_shares, blockIdx.x - p.tiles,
+                      gridDim.x - p.tiles);
+  const uint32_t e0 = blockIdx.x * kThreads * kItems + threadIdx.x;
+  uint32_t key[kItems];
+#pragma unroll
+  for (int i = 0; i < kItems; ++i)
+    if (e0 + i * kThreads < p.n) key[i] = load_key(p, e0 + i * kThreads);
+#pragma unroll
+  for (int i = 0; i < kItems; ++i)
+    if (e0 + i * kThreads < p.n) atomicAdd(&count[(key[i] >> p.shift) & ((1u << p.bits) - 1)], 1u);
+  __syncthreads();
+  for (uint32_t d = threadIdx.x; d < p.bins; d += kThreads)
+    p.counts[(uint64_t)d * p.tiles + blockIdx.x] = count[d];
+}
+
+template <int kItems, bool kExperts>
 __global__ void __launch_bounds__(kThreads) tile_place_kernel(Pass p, ExpertOut o) {
-  __shared__ uint16_t seen[kWarps][kMaxBins];  // at most 32 * kItems a warp
-  __shared__ uint32_t base[kMaxBins];
+  constexpr uint32_t kBins = 1 << (kExperts ? kExpertBits : kTokenBits);
+  __shared__ Seen<kBins> seen;
+  __shared__ uint32_t base[kBins], all[kBins];
   __shared__ uint32_t warp_sum[kWarps];
   pdl_trigger_at_entry();
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (uint32_t d = lane; d < p.bins; d += 32) seen[warp][d] = 0;
+  clear_seen(seen, p.bins);
   __syncwarp();
   pdl_wait();
   pdl_launch_dependents();
-  const uint32_t e0 = blockIdx.x * kTile + warp * 32 * kItems + lane;
-  uint32_t key[kItems], rank[kItems];
+  if (blockIdx.x >= p.tiles)
+    return zero_share(p.fill, p.fill_share, p.fill_shares, blockIdx.x - p.tiles,
+                      gridDim.x - p.tiles);
+  const uint32_t e0 = (blockIdx.x * kThreads + warp * 32) * kItems + lane;
+  uint32_t key[kItems], digit[kItems], rank[kItems];
 #pragma unroll
   for (int i = 0; i < kItems; ++i) {
-    const uint32_t e = e0 + i * 32;
-    key[i] = e < p.n ? load_key(p, e) : 0;
+    key[i] = e0 + i * 32 < p.n ? load_key(p, e0 + i * 32) : 0;
+    digit[i] = (key[i] >> p.shift) & ((1u << p.bits) - 1);
   }
+  rank_in_warp(seen, digit, e0, p.n, rank);
+  if (p.tiles > 1) {  // a warp adds up a digit's row of counts, four digits at a time
+    for (uint32_t d0 = warp; d0 < p.bins; d0 += 4 * kWarps) {
+      uint32_t sum[4] = {}, earlier[4] = {};
+      for (uint32_t t = lane; t < p.tiles; t += 32) {
 #pragma unroll
-  for (int i = 0; i < kItems; ++i) {
-    const bool in = e0 + i * 32 < p.n;
-    const uint32_t lanes = __ballot_sync(~0u, in);
-    if (in) {
-      const uint32_t d = (key[i] >> p.shift) & (kMaxBins - 1);
-      const uint32_t same = __match_any_sync(lanes, d);
-      const uint32_t before = seen[warp][d];
-      __syncwarp(lanes);
-      rank[i] = before + __popc(same & ((1u << lane) - 1));
-      if ((same >> lane) == 1) seen[warp][d] = (uint16_t)(before + __popc(same));
-      __syncwarp(lanes);
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t d = d0 + j * kWarps;
+          const uint32_t c = d < p.bins ? p.counts[(uint64_t)d * p.tiles + t] : 0;
+          sum[j] += c;
+          if (t < blockIdx.x) earlier[j] += c;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t d = d0 + j * kWarps;
+        const uint32_t s = __reduce_add_sync(~0u, sum[j]), b = __reduce_add_sync(~0u, earlier[j]);
+        if (lane == 0 && d < p.bins) all[d] = s, base[d] = b;
+      }
     }
   }
   __syncthreads();
-  // A thread takes the digits d = threadIdx.x and threadIdx.x + kThreads in turn.
   uint32_t carry = 0;
   for (uint32_t d0 = 0; d0 < p.bins; d0 += kThreads) {
     const uint32_t d = d0 + threadIdx.x;
-    uint32_t all = 0, earlier = 0;
+    uint32_t mine = 0, earlier = 0, room = 0, total;
     if (d < p.bins) {
-      uint32_t run = 0;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const uint32_t c = seen[w][d];
-        seen[w][d] = (uint16_t)run;
-        run += c;
-      }
-      if (p.tiles == 1) {
-        all = run;
-      } else {
-        for (uint32_t t = 0; t < p.tiles; ++t) {
-          const uint32_t c = p.counts[t * p.bins + d];
-          if (t < blockIdx.x) earlier += c;
-          all += c;
-        }
-      }
-    }
-    uint32_t room = all, total;
-    if (kExperts) {  // the last digit holds the entries without an expert
-      room = d + 1 < p.bins ? (all + o.align - 1) / o.align * o.align : 0;
+      mine = sum_over_warps(seen, d);
+      if (p.tiles > 1) mine = all[d], earlier = base[d];
+      room = mine;
+      if (kExperts)  // the last digit holds the entries without an expert
+        room = d + 1 < p.bins ? (mine + o.align - 1) / o.align * o.align : 0;
     }
     const uint32_t at = carry + block_exclusive(room, warp_sum, &total);
     carry += total;
@@ -161,21 +246,20 @@ __global__ void __launch_bounds__(kThreads) tile_place_kernel(Pass p, ExpertOut 
       if (kExperts) {
         if (blockIdx.x == 0) o.offsets[d] = (int32_t)at;  // the last one: all rows in use
         if (d + 1 < p.bins)
-          for (uint32_t r = at + all + blockIdx.x; r < at + room; r += gridDim.x) o.source[r] = -1;
+          for (uint32_t r = at + mine + blockIdx.x; r < at + room; r += p.tiles) o.source[r] = -1;
       }
     }
   }
   if (kExperts)
     for (uint32_t r = carry + blockIdx.x * kThreads + threadIdx.x; r < o.rows;
-         r += gridDim.x * kThreads)
+         r += p.tiles * kThreads)
       o.source[r] = -1;
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kItems; ++i) {
-    const uint32_t e = e0 + i * 32;
+    const uint32_t e = e0 + i * 32, d = digit[i];
     if (e >= p.n) continue;
-    const uint32_t d = (key[i] >> p.shift) & (kMaxBins - 1);
-    const uint32_t to = base[d] + seen[warp][d] + rank[i];
+    const uint32_t to = base[d] + seen.of[warp][d] + rank[i];
     if (kExperts) {
       const bool kept = d + 1 < p.bins;
       o.dest[e] = kept ? (int32_t)to : -1;
@@ -187,16 +271,99 @@ __global__ void __launch_bounds__(kThreads) tile_place_kernel(Pass p, ExpertOut 
   }
 }
 
-uint32_t tiles_of(uint64_t n) { return (uint32_t)((n + kTile - 1) / kTile); }
+// All digits of at most kItems * kThreads entries in one block.
+template <int kItems>
+__global__ void __launch_bounds__(kThreads) one_tile_kernel(Pass p) {
+  constexpr uint32_t kRoom = kItems * kThreads, kBins = 1 << kTokenBits;
+  __shared__ Seen<kBins> seen;
+  __shared__ uint32_t keys[kRoom], base[kBins], warp_sum[kWarps];
+  __shared__ uint16_t places[kRoom];
+  pdl_trigger_at_entry();
+  pdl_wait();
+  pdl_launch_dependents();
+  if (blockIdx.x >= 1) return zero_share(p.fill, 0, 1, blockIdx.x - 1, gridDim.x - 1);
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t e0 = warp * 32 * kItems + lane, bins = 1u << p.bits;
+  uint32_t key[kItems], place[kItems], digit[kItems], rank[kItems];
+#pragma unroll
+  for (int i = 0; i < kItems; ++i) {
+    place[i] = e0 + i * 32;
+    key[i] = place[i] < p.n ? entry_key(p.src, place[i]) : 0;
+  }
+  for (uint32_t pass = 0; pass < p.passes; ++pass) {
+    clear_seen(seen, bins);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) digit[i] = (key[i] >> (pass * p.bits)) & (bins - 1);
+    rank_in_warp(seen, digit, e0, p.n, rank);
+    __syncthreads();
+    uint32_t carry = 0;
+    for (uint32_t d0 = 0; d0 < bins; d0 += kThreads) {
+      const uint32_t d = d0 + threadIdx.x;
+      const uint32_t mine = d < bins ? sum_over_warps(seen, d) : 0;
+      uint32_t total;
+      const uint32_t at = carry + block_exclusive(mine, warp_sum, &total);
+      carry += total;
+      if (d < bins) base[d] = at;
+    }
+    __syncthreads();
+    const bool last = pass + 1 == p.passes;
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+      if (e0 + i * 32 >= p.n) continue;
+      const uint32_t to = base[digit[i]] + seen.of[warp][digit[i]] + rank[i];
+      if (last) p.key_out[to] = key[i], p.pos_out[to] = place[i];
+      else keys[to] = key[i], places[to] = (uint16_t)place[i];
+    }
+    if (last) return;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kItems; ++i)
+      if (e0 + i * 32 < p.n) key[i] = keys[e0 + i * 32], place[i] = places[e0 + i * 32];
+  }
+}
+
+// Entries a thread ranks.  Few keep many tiles (SMs) at work, many keep the tiles'
+// counts, which every tile reads, below the entries: 131072 entries are sorted in 10 us
+// with 2 and 15 us with 8.
+int items_of(uint64_t n) { return n <= 128 * 2 * kThreads ? 2 : n <= 1024 * 8 * kThreads ? 8 : 32; }
+uint32_t tiles_of(uint64_t n) {
+  const uint64_t tile = (uint64_t)items_of(n) * kThreads;
+  return (uint32_t)((n + tile - 1) / tile);
+}
+
+template <typename F>
+int with_items(int items, F &&f) {
+  if (items == 2) return f(std::integral_constant<int, 2>{});
+  if (items == 8) return f(std::integral_constant<int, 8>{});
+  return f(std::integral_constant<int, 32>{});
+}
+
+uint32_t fill_blocks(const Fill &f) {
+  const uint64_t bytes = f.rows * f.bytes;
+  return (uint32_t)std::min<uint64_t>((bytes + kThreads * 64 - 1) / (kThreads * 64),
+                                      4ull * sm_count());
+}
+
+__global__ void __launch_bounds__(kThreads) zero_kernel(Fill f) {
+  pdl_trigger_at_entry();
+  pdl_wait();
+  pdl_launch_dependents();
+  zero_share(f, 0, 1, blockIdx.x, gridDim.x);
+}
 
 }  // namespace
 
-uint64_t sort_by_key_bytes(uint64_t n, uint64_t keys) {
-  (void)keys;
-  return 4 * n * sizeof(uint32_t) + (uint64_t)tiles_of(n) * kMaxBins * sizeof(uint32_t);
+int fill_zero(const Fill &fill, cudaStream_t s) {
+  if (fill_blocks(fill) == 0) return DCOPY_OK;
+  return launch(zero_kernel, fill_blocks(fill), dim3(kThreads), 0, s, "zero_kernel", fill);
 }
 
-int sort_by_key(const KeySource &src, void *workspace, const uint32_t **key_out,
+uint64_t sort_by_key_bytes(uint64_t n) {
+  return (4 * n + ((uint64_t)tiles_of(n) << kTokenBits)) * sizeof(uint32_t);
+}
+
+int sort_by_key(const KeySource &src, const Fill &fill, void *workspace, const uint32_t **key_out,
                 const uint32_t **pos_out, cudaStream_t s) {
   uint32_t *w = static_cast<uint32_t *>(workspace);
   uint32_t *key[2] = {w, w + 2ull * src.n}, *pos[2] = {w + src.n, w + 3ull * src.n};
@@ -204,22 +371,40 @@ int sort_by_key(const KeySource &src, void *workspace, const uint32_t **key_out,
   p.src = src;
   p.counts = w + 4ull * src.n;
   p.n = src.n;
+  p.fill = fill;
+  uint32_t key_bits = 1;  // keys themselves occur, as the key of what belongs nowhere
+  while (key_bits < 32 && src.keys >> key_bits) ++key_bits;
+  p.passes = (key_bits + kTokenBits - 1) / kTokenBits;
+  p.bits = (key_bits + p.passes - 1) / p.passes;
+  const uint32_t fills = fill_blocks(fill);
+  if (src.n <= kOneTile) {
+    p.key_out = key[0];
+    p.pos_out = pos[0];
+    *key_out = key[0];
+    *pos_out = pos[0];
+    auto k = src.n <= 2 * kThreads ? one_tile_kernel<2> : one_tile_kernel<8>;
+    return launch(k, 1 + fills, dim3(kThreads), 0, s, "one_tile_kernel", p);
+  }
   p.tiles = tiles_of(src.n);
-  int to = 0;
-  for (uint32_t shift = 0; shift == 0 || (shift < 32 && src.keys >> shift != 0); shift += 10) {
-    p.shift = shift;
-    p.bins = std::min<uint32_t>(kMaxBins, (src.keys >> shift) + 1);
-    p.key_out = key[to];
-    p.pos_out = pos[to];
-    if (p.tiles > 1)
-      if (int rc = launch(tile_count_kernel, p.tiles, dim3(kThreads), 0, s, "tile_count_kernel", p))
+  p.fill_shares = 2 * p.passes;
+  for (uint32_t pass = 0; pass < p.passes; ++pass) {
+    p.shift = pass * p.bits;
+    p.bins = std::min<uint32_t>(1u << p.bits, (src.keys >> p.shift) + 1);
+    p.key_out = key[pass & 1];
+    p.pos_out = pos[pass & 1];
+    const int rc = with_items(items_of(src.n), [&](auto items) {
+      constexpr int kItems = decltype(items)::value;
+      p.fill_share = 2 * pass;
+      if (int rc = launch(tile_count_kernel<kItems>, p.tiles + fills, dim3(kThreads), 0, s,
+                          "tile_count_kernel", p))
         return rc;
-    if (int rc = launch(tile_place_kernel<false>, p.tiles, dim3(kThreads), 0, s,
-                        "tile_place_kernel", p, ExpertOut{}))
-      return rc;
-    p.key_in = key[to];
-    p.pos_in = pos[to];
-    to ^= 1;
+      p.fill_share = 2 * pass + 1;
+      return launch(tile_place_kernel<kItems, false>, p.tiles + fills, dim3(kThreads), 0, s,
+                    "tile_place_kernel", p, ExpertOut{});
+    });
+    if (rc) return rc;
+    p.key_in = p.key_out;
+    p.pos_in = p.pos_out;
   }
   *key_out = p.key_in;
   *pos_out = p.pos_in;
@@ -227,8 +412,7 @@ int sort_by_key(const KeySource &src, void *workspace, const uint32_t **key_out,
 }
 
 uint64_t sort_experts_bytes(uint64_t n, uint32_t experts) {
-  const uint32_t tiles = tiles_of(n);
-  return tiles > 1 ? (uint64_t)tiles * (experts + 1) * sizeof(uint32_t) : 0;
+  return n <= kOneTile ? 0 : (uint64_t)tiles_of(n) * (experts + 1) * sizeof(uint32_t);
 }
 
 int sort_experts(const KeySource &src, uint32_t align, int32_t *dest, int32_t *source,
@@ -237,13 +421,20 @@ int sort_experts(const KeySource &src, uint32_t align, int32_t *dest, int32_t *s
   p.src = src;
   p.counts = static_cast<uint32_t *>(workspace);
   p.n = src.n;
-  p.tiles = std::max<uint32_t>(1, tiles_of(src.n));
   p.bins = src.keys + 1;
-  if (p.tiles > 1)
-    if (int rc = launch(tile_count_kernel, p.tiles, dim3(kThreads), 0, s, "tile_count_kernel", p))
-      return rc;
-  return launch(tile_place_kernel<true>, p.tiles, dim3(kThreads), 0, s, "tile_place_kernel", p,
-                ExpertOut{dest, source, offsets, align, rows});
+  p.bits = kExpertBits;
+  const bool one = src.n <= kOneTile;
+  const int most = one ? (src.n <= 2 * kThreads ? 2 : 8) : items_of(src.n);
+  p.tiles = one ? 1 : tiles_of(src.n);
+  return with_items(most, [&](auto items) {
+    constexpr int kItems = decltype(items)::value;
+    if (!one)
+      if (int rc = launch(tile_count_kernel<kItems>, p.tiles, dim3(kThreads), 0, s,
+                          "tile_count_kernel", p))
+        return rc;
+    return launch(tile_place_kernel<kItems, true>, p.tiles, dim3(kThreads), 0, s,
+                  "tile_place_kernel", p, ExpertOut{dest, source, offsets, align, rows});
+  });
 }
 
 }  // namespace dcopy

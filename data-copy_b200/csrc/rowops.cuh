@@ -66,14 +66,13 @@ inline int check_apart(const DcopyMatrix *a, const DcopyMatrix *b, const char *w
   return check_disjoint(a->data, matrix_span(a), b->data, matrix_span(b), what);
 }
 
-// Largest V in {8, 4, 2, 1} for which a row of the matrix is whole vectors of V
-// elements that start on the vector's own alignment (16 bytes at most).
-inline int vector_width(const DcopyMatrix *m, int most = 8) {
+// Largest V in {8, 4, 2, 1} of at most 16 bytes for which a row of the matrix is whole
+// vectors of V elements that start on the vector's own alignment.
+inline int vector_width(const DcopyMatrix *m) {
   const int eb = elem_size(m->type);
-  for (int v = most; v > 1; v /= 2) {
-    const int align = std::min(16, v * eb);
-    if (m->cols % v == 0 && reinterpret_cast<uintptr_t>(m->data) % align == 0 &&
-        (m->rows <= 1 || (uint64_t)m->pitch * eb % align == 0))
+  for (int v = 16 / eb; v > 1; v /= 2) {
+    if (m->cols % v == 0 && reinterpret_cast<uintptr_t>(m->data) % (v * eb) == 0 &&
+        (m->rows <= 1 || (uint64_t)m->pitch * eb % (v * eb) == 0))
       return v;
   }
   return 1;
@@ -167,6 +166,23 @@ struct Words {
       *reinterpret_cast<uint8_t *>(p) = (uint8_t)w[0];
     }
   }
+  // The same marked as written once and not read soon: L2 evicts it first.
+  __device__ __forceinline__ void store_cs(void *p) const {
+    if constexpr (N >= 16) {
+#pragma unroll
+      for (int i = 0; i < N / 16; ++i)
+        __stcs(reinterpret_cast<uint4 *>(p) + i,
+               make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]));
+    } else if constexpr (N == 8) {
+      __stcs(reinterpret_cast<uint2 *>(p), make_uint2(w[0], w[1]));
+    } else if constexpr (N == 4) {
+      __stcs(reinterpret_cast<uint32_t *>(p), w[0]);
+    } else if constexpr (N == 2) {
+      __stcs(reinterpret_cast<unsigned short *>(p), (unsigned short)w[0]);
+    } else {
+      __stcs(reinterpret_cast<unsigned char *>(p), (unsigned char)w[0]);
+    }
+  }
   __device__ __forceinline__ void zero() {
 #pragma unroll
     for (int i = 0; i < kWords; ++i) w[i] = 0;
@@ -209,10 +225,11 @@ struct RowSplit {
   dim3 grid;
 };
 
-inline RowSplit split_rows(uint64_t rows, uint64_t vectors, int u) {
+inline RowSplit split_rows(uint64_t rows, uint64_t vectors, int u, int most_rows = kRowThreads) {
   RowSplit s;
   s.lx = 0;
-  while ((1 << s.lx) < kRowThreads && (1ull << s.lx) < vectors) ++s.lx;
+  while (kRowThreads >> s.lx > most_rows) ++s.lx;
+  while ((1 << s.lx) < kRowThreads && ((uint64_t)u << s.lx) < vectors) ++s.lx;
   const uint64_t per_block = kRowThreads >> s.lx, step = (uint64_t)u << s.lx;
   s.grid = dim3((unsigned)((rows + per_block - 1) / per_block),
                 (unsigned)((vectors + step - 1) / step));
