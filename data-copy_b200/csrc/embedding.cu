@@ -69,8 +69,16 @@ __global__ void __launch_bounds__(kRowThreads) lookup_kernel(Lookup p) {
 
 // ---- gradient -------------------------------------------------------------------
 
-constexpr uint32_t kPiece = 32;      // sorted entries of a piece
+// Sorted entries of a piece: 32 where there are enough pieces for all SMs (16384
+// tokens: 199 us against 206 with 16), 16 below (2047 tokens: 30 us against 34 with 32).
+constexpr uint32_t kPiece = 32, kSmallPiece = 16, kFewTokens = 4096;
 constexpr uint32_t kMaxPieces = 32;  // pieces of a block
+// Bytes zeroed beside the joining of runs, and by a block: small blocks spread a small
+// fill over the SMs (36 MB: 30 us with 32 KB, 46 with 128 KB), large ones search less
+// often for the rows that tokens have (800 MB: 199 us with 128 KB, 232 with 32 KB).
+constexpr uint64_t kFillLate = 32ull << 20;
+constexpr uint64_t kFillBlockLeast = 32ull << 10, kFillBlockMost = 128ull << 10;
+constexpr uint64_t kFillBlocks = 2048;
 
 struct Grad {
   void *grad;
@@ -78,10 +86,51 @@ struct Grad {
   int64_t grad_pitch, dout_pitch;
   const uint32_t *key, *pos;  // in key order
   float *head, *tail;         // [pieces][width] sums of runs that cross piece ends
-  uint32_t n, keys, pieces, vectors, width;
+  uint32_t n, keys, piece, pieces, vectors, width;  // piece: entries of one
   int lx;
   float scale;
+  Fill fill;                  // rows to zero where no token has them
+  uint32_t piece_blocks, work_blocks, fill_rows;  // a block's pieces x columns, then the fill
 };
+
+// Blocks behind a kernel's own: fill_rows rows each of the fill, but those that some
+// token has, which the sums are written to.  The place of the first row in the sorted
+// ids is found by a search that narrows by the block's size a step.
+__device__ __forceinline__ void zero_untouched(const Grad &p, uint32_t block) {
+  __shared__ uint32_t touched[kRowThreads / 32];
+  const uint64_t row0 = p.fill.begin + (uint64_t)block * p.fill_rows;
+  const uint64_t row1 = min(row0 + p.fill_rows, p.fill.end);
+  if (threadIdx.x < kRowThreads / 32) touched[threadIdx.x] = 0;
+  uint32_t lo = 0, length = p.n;  // the first entry not below row0 lies in [lo, lo + length]
+  while (length > 0) {
+    const uint32_t step = (length + kRowThreads - 1) / kRowThreads;
+    const uint32_t i = threadIdx.x * step;
+    const uint32_t below = __syncthreads_count(i < length && p.key[lo + i] < row0);
+    if (below == 0) break;  // lo itself
+    const uint32_t from = (below - 1) * step + 1;  // the entry before it is below row0
+    const uint32_t to = min(below * step, length);
+    lo += from;
+    length = to - from;
+  }
+  __syncthreads();
+  for (uint32_t i0 = lo; i0 < p.n; i0 += kRowThreads) {
+    const uint32_t key = i0 + threadIdx.x < p.n ? p.key[i0 + threadIdx.x] : p.keys;
+    const bool in = key < row1;
+    if (in) atomicOr(&touched[(key - (uint32_t)row0) / 32], 1u << (key - (uint32_t)row0) % 32);
+    if (!__syncthreads_and(in)) break;
+  }
+  __syncthreads();
+  uint32_t any = 0;
+  for (uint32_t w = 0; w < kRowThreads / 32; ++w) any |= touched[w];
+  if (!any && p.fill.pitch == p.fill.bytes)
+    return zero_bytes(p.fill.dst + row0 * p.fill.pitch, (row1 - row0) * p.fill.bytes, threadIdx.x,
+                      kRowThreads);
+  for (uint64_t r = row0 + threadIdx.x / 32; r < row1; r += kRowThreads / 32) {
+    const uint32_t k = (uint32_t)(r - row0);
+    if (!(touched[k / 32] >> k % 32 & 1))
+      zero_bytes(p.fill.dst + r * p.fill.pitch, p.fill.bytes, threadIdx.x % 32, 32);
+  }
+}
 
 template <typename T, int V, bool kAdd>
 __device__ __forceinline__ void write_row(T *row, uint32_t c, const float (&sum)[V], float scale) {
@@ -109,18 +158,21 @@ __global__ void __launch_bounds__(kRowThreads) piece_sum_kernel(Grad p) {
   pdl_trigger_at_entry();
   pdl_wait();
   pdl_launch_dependents();
+  if (blockIdx.x >= p.work_blocks) return zero_untouched(p, blockIdx.x - p.work_blocks);
+  const uint32_t by = blockIdx.x / p.piece_blocks, bx = blockIdx.x - by * p.piece_blocks;
   const uint32_t block_pieces = kRowThreads >> p.lx;
-  const uint32_t first = blockIdx.x * block_pieces * kPiece;  // entry
-  for (uint32_t i = threadIdx.x; i < block_pieces * kPiece + 2; i += kRowThreads) {
+  const uint32_t first = bx * block_pieces * p.piece;  // entry
+  for (uint32_t i = threadIdx.x; i < block_pieces * p.piece + 2; i += kRowThreads) {
     const uint32_t e = first + i;  // entry e - 1
     keys[i] = e >= 1 && e <= p.n ? p.key[e - 1] : p.keys;
-    if (i >= 1 && i <= block_pieces * kPiece && e <= p.n) places[i - 1] = p.pos[e - 1];
+    if (i >= 1 && i <= block_pieces * p.piece && e <= p.n) places[i - 1] = p.pos[e - 1];
   }
   __syncthreads();
-  const uint32_t local = (threadIdx.x >> p.lx) * kPiece, piece = first / kPiece + (threadIdx.x >> p.lx);
-  const uint32_t c = (blockIdx.y << p.lx) + (threadIdx.x & ((1u << p.lx) - 1));
+  const uint32_t local = (threadIdx.x >> p.lx) * p.piece;
+  const uint32_t piece = bx * block_pieces + (threadIdx.x >> p.lx);
+  const uint32_t c = (by << p.lx) + (threadIdx.x & ((1u << p.lx) - 1));
   if (piece >= p.pieces || c >= p.vectors) return;
-  const uint32_t count = min(kPiece, p.n - piece * kPiece);
+  const uint32_t count = min(p.piece, p.n - piece * p.piece);
   const TIn *dout = static_cast<const TIn *>(p.dout) + (uint64_t)c * V;
   TOut *grad = static_cast<TOut *>(p.grad);
   uint32_t key = keys[local + 1];
@@ -164,10 +216,12 @@ __global__ void __launch_bounds__(kRowThreads) piece_join_kernel(Grad p) {
   pdl_trigger_at_entry();
   pdl_wait();
   pdl_launch_dependents();
-  const uint32_t piece = blockIdx.x * (kRowThreads >> p.lx) + (threadIdx.x >> p.lx);
-  const uint32_t c = (blockIdx.y << p.lx) + (threadIdx.x & ((1u << p.lx) - 1));
+  if (blockIdx.x >= p.work_blocks) return zero_untouched(p, blockIdx.x - p.work_blocks);
+  const uint32_t by = blockIdx.x / p.piece_blocks, bx = blockIdx.x - by * p.piece_blocks;
+  const uint32_t piece = bx * (kRowThreads >> p.lx) + (threadIdx.x >> p.lx);
+  const uint32_t c = (by << p.lx) + (threadIdx.x & ((1u << p.lx) - 1));
   if (piece + 1 >= p.pieces || c >= p.vectors) return;
-  const uint32_t b = piece * kPiece, last = b + kPiece - 1;
+  const uint32_t b = piece * p.piece, last = b + p.piece - 1;
   const uint32_t key = p.key[last];
   if (key >= p.keys || p.key[last + 1] != key) return;    // nothing goes on
   if (p.key[b] == key && b > 0 && p.key[b - 1] == key) return;  // it began earlier
@@ -184,7 +238,7 @@ __global__ void __launch_bounds__(kRowThreads) piece_join_kernel(Grad p) {
     bool same[kAhead];
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
-      same[j] = q + j < p.pieces && p.key[(q + j) * kPiece] == key;
+      same[j] = q + j < p.pieces && p.key[(q + j) * p.piece] == key;
       if (q + j < p.pieces) head[j].load(p.head + (uint64_t)(q + j) * p.width + at);
     }
 #pragma unroll
@@ -214,7 +268,8 @@ int id_source(const DcopyMatrix *ids, int64_t first, int64_t keys, KeySource *sr
   return DCOPY_OK;
 }
 
-uint64_t pieces_of(uint64_t n) { return (n + kPiece - 1) / kPiece; }
+uint32_t piece_of(uint64_t n) { return n <= kFewTokens ? kSmallPiece : kPiece; }
+uint64_t pieces_of(uint64_t n) { return (n + piece_of(n) - 1) / piece_of(n); }
 
 }  // namespace
 }  // namespace dcopy
@@ -251,7 +306,7 @@ int dcopy_embedding_lookup(const DcopyMatrix *out, const DcopyMatrix *table,
     return with_float(out->type, [&](auto tout) {
       using TIn = typename decltype(tin)::type;
       using TOut = typename decltype(tout)::type;
-      return with_vector(std::min(vector_width(out), vector_width(table)), [&](auto vw) {
+      return with_vector<std::max(sizeof(TIn), sizeof(TOut))>(std::min(vector_width(out), vector_width(table)), [&](auto vw) {
         constexpr int V = decltype(vw)::value;
         p.vectors = (uint32_t)(out->cols / V);
         const bool many = (uint64_t)p.ids.n * p.vectors >= (uint64_t)sm_count() * 2048 * 4;
@@ -309,22 +364,22 @@ int dcopy_embedding_grad(const DcopyMatrix *grad, const DcopyMatrix *dout, const
   if (!accumulate) {
     const uint64_t eb = elem_size(grad->type);
     fill.dst = static_cast<uint8_t *>(grad->data);
-    fill.rows = grad->rows;
+    fill.end = grad->rows;
     fill.bytes = grad->cols * eb;
     fill.pitch = grad->pitch * eb;
-    if (fill.rows == 1 || fill.pitch == fill.bytes) fill.bytes *= fill.rows, fill.rows = 1;
   }
   if (src.n == 0) return fill_zero(fill, stream);
   uint8_t *ws = reinterpret_cast<uint8_t *>(((uintptr_t)workspace + 15) / 16 * 16);
   const uint64_t sort = (sort_by_key_bytes(src.n) + 15) / 16 * 16;
   Grad p{};
-  if (int rc = sort_by_key(src, fill, ws, &p.key, &p.pos, stream)) return rc;
+  if (int rc = sort_by_key(src, &fill, ws, &p.key, &p.pos, stream)) return rc;
   p.grad = grad->data;
   p.dout = dout->data;
   p.grad_pitch = grad->pitch;
   p.dout_pitch = dout->pitch;
   p.n = src.n;
   p.keys = src.keys;
+  p.piece = piece_of(src.n);
   p.pieces = (uint32_t)pieces_of(src.n);
   p.width = (uint32_t)((grad->cols + 3) / 4 * 4);
   p.head = reinterpret_cast<float *>(ws + sort);
@@ -334,7 +389,7 @@ int dcopy_embedding_grad(const DcopyMatrix *grad, const DcopyMatrix *dout, const
     return with_float(grad->type, [&](auto tout) {
       using TIn = typename decltype(tin)::type;
       using TOut = typename decltype(tout)::type;
-      return with_vector(std::min(vector_width(dout), vector_width(grad)), [&](auto vw) {
+      return with_vector<std::max(sizeof(TIn), sizeof(TOut))>(std::min(vector_width(dout), vector_width(grad)), [&](auto vw) {
         constexpr int V = decltype(vw)::value;
         p.vectors = (uint32_t)(grad->cols / V);
         const RowSplit split = split_rows(p.pieces, p.vectors, 1, kMaxPieces);
@@ -342,10 +397,27 @@ int dcopy_embedding_grad(const DcopyMatrix *grad, const DcopyMatrix *dout, const
         auto sum = accumulate ? piece_sum_kernel<TIn, TOut, V, true>
                               : piece_sum_kernel<TIn, TOut, V, false>;
         auto join = accumulate ? piece_join_kernel<TOut, V, true> : piece_join_kernel<TOut, V, false>;
-        if (int rc = launch_grid(sum, split.grid, dim3(kRowThreads), 0, stream, "piece_sum_kernel", p))
-          return rc;
-        if (p.pieces == 1) return DCOPY_OK;
-        return launch_grid(join, split.grid, dim3(kRowThreads), 0, stream, "piece_join_kernel", p);
+        // What is left to zero goes along with the two launches: as much with the second
+        // as hides the latency of its few long runs, the rest with the first.
+        const uint64_t left = fill.bytes ? fill.end - fill.begin : 0;
+        const uint64_t late = std::min<uint64_t>(
+            left, p.pieces > 1 && left ? std::max<uint64_t>(1, kFillLate / fill.bytes) : 0);
+        auto step = [&](auto kernel, const char *name, uint64_t rows) {
+          p.fill = fill;
+          const uint64_t block = std::clamp<uint64_t>(rows * fill.bytes / kFillBlocks,
+                                                      kFillBlockLeast, kFillBlockMost);
+          if (rows)
+            p.fill_rows = (uint32_t)std::clamp<uint64_t>(block / fill.bytes, 1, kRowThreads);
+          p.fill.begin = fill.end - rows;
+          fill.end -= rows;
+          p.piece_blocks = split.grid.x;
+          p.work_blocks = split.grid.x * split.grid.y;
+          const uint32_t fills = rows ? (uint32_t)((rows + p.fill_rows - 1) / p.fill_rows) : 0;
+          return launch(kernel, p.work_blocks + fills, dim3(kRowThreads), 0, stream, name, p);
+        };
+        if (int rc = step(sum, "piece_sum_kernel", left - late)) return rc;
+        if (p.pieces == 1) return (int)DCOPY_OK;
+        return step(join, "piece_join_kernel", late);
       });
     });
   });

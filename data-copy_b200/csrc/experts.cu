@@ -337,7 +337,7 @@ int dcopy_expert_dispatch(const DcopyMatrix *out, const DcopyMatrix *x, const in
     p.in_pitch = x->pitch;
     return with_float(out->type, [&](auto t) {
       using T = typename decltype(t)::type;
-      return with_vector(std::min(vector_width(out), vector_width(x)), [&](auto vw) {
+      return with_vector<sizeof(T)>(std::min(vector_width(out), vector_width(x)), [&](auto vw) {
         constexpr int V = decltype(vw)::value;
         p.vectors = (uint32_t)(out->cols / V);
         RowSplit split = split_rows(p.tokens, p.vectors, 1);
@@ -395,7 +395,7 @@ int dcopy_expert_combine(const DcopyMatrix *out, const DcopyMatrix *y, const int
   p.rows = (uint32_t)y->rows;
   return with_float(out->type, [&](auto t) {
     using T = typename decltype(t)::type;
-    return with_vector(std::min(vector_width(out), vector_width(y)), [&](auto vw) {
+    return with_vector<sizeof(T)>(std::min(vector_width(out), vector_width(y)), [&](auto vw) {
       constexpr int V = decltype(vw)::value;
       p.vectors = (uint32_t)(out->cols / V);
       const RowSplit split = split_rows(p.tokens, p.vectors, 1);
@@ -452,7 +452,7 @@ int dcopy_expert_combine_grad(const DcopyMatrix *dy, const DcopyMatrix *dweights
   return with_float(dy->type, [&](auto t) {
     using T = typename decltype(t)::type;
     const int v = std::min(std::min(vector_width(dy), vector_width(dout)), vector_width(y));
-    return with_vector(v, [&](auto vw) {
+    return with_vector<sizeof(T)>(v, [&](auto vw) {
       constexpr int V = decltype(vw)::value;
       p.vectors = (uint32_t)(dy->cols / V);
       return launch_grid(combine_grad_kernel<T, V>, dim3(blocks), dim3(kRowThreads), 0, stream,

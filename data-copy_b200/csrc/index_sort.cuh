@@ -21,20 +21,21 @@ struct KeySource {
   FastDiv cols;
 };
 
-// Memory to zero beside the sort: its few blocks leave most SMs idle, so each of its
-// launches also clears a share.  16-byte granules, `pitch` apart by rows (one row:
-// contiguous), and the bytes at the ends that no whole granule covers.
+// Rows [begin, end) to zero beside the sort: its few blocks leave most SMs idle, so
+// each of its launches also clears some, the last ones first.  (Vocabularies have their
+// frequent ids in front, and rows that tokens have are written again.)
 struct Fill {
   uint8_t *dst = nullptr;
   uint64_t pitch = 0, bytes = 0;  // of a row
-  uint64_t rows = 0;
+  uint64_t begin = 0, end = 0;
 };
 
 // Workspace bytes of sort_by_key for n entries.
 uint64_t sort_by_key_bytes(uint64_t n);
 // key_out[p], pos_out[p]: the p-th entry in key order, equal keys in entry order.
-// Both arrays (n values each) lie in the workspace.  n is at least 1.
-int sort_by_key(const KeySource &src, const Fill &fill, void *workspace, const uint32_t **key_out,
+// Both arrays (n values each) lie in the workspace.  n is at least 1.  fill becomes
+// the rows that are left.
+int sort_by_key(const KeySource &src, Fill *fill, void *workspace, const uint32_t **key_out,
                 const uint32_t **pos_out, cudaStream_t s);
 // Clears alone.
 int fill_zero(const Fill &fill, cudaStream_t s);

@@ -236,15 +236,28 @@ inline RowSplit split_rows(uint64_t rows, uint64_t vectors, int u, int most_rows
   return s;
 }
 
-// Calls f with a value of type std::integral_constant<int, V> for V in {8, 4, 2, 1}.
-template <typename F>
+// Calls f with a value of type std::integral_constant<int, V> for the vector width v
+// (as vector_width gives it) of elements of at most kBytes bytes.
+template <int kBytes, typename F>
 int with_vector(int v, F &&f) {
-  switch (v) {
-    case 8: return f(std::integral_constant<int, 8>{});
-    case 4: return f(std::integral_constant<int, 4>{});
-    case 2: return f(std::integral_constant<int, 2>{});
-    default: return f(std::integral_constant<int, 1>{});
-  }
+  if constexpr (kBytes <= 2)
+    if (v == 8) return f(std::integral_constant<int, 8>{});
+  if (v == 4) return f(std::integral_constant<int, 4>{});
+  if (v == 2) return f(std::integral_constant<int, 2>{});
+  return f(std::integral_constant<int, 1>{});
+}
+
+// Zeroes `bytes` bytes by the threads `t` of `threads`: 16-byte granules, bytes at the
+// ends.
+__device__ __forceinline__ void zero_bytes(uint8_t *at, uint64_t bytes, uint32_t t,
+                                           uint32_t threads) {
+  const uint64_t head = min((uint64_t)(-(uintptr_t)at & 15), bytes);
+  const uint64_t units = (bytes - head) / 16, tail = bytes - head - units * 16;
+  uint4 *dst = reinterpret_cast<uint4 *>(at + head);
+#pragma unroll 4
+  for (uint64_t u = t; u < units; u += threads) dst[u] = make_uint4(0, 0, 0, 0);
+  if (t < head) at[t] = 0;
+  if (t < tail) at[bytes - 1 - t] = 0;
 }
 
 template <typename T>
