@@ -29,6 +29,7 @@ struct Route {
   const int32_t *dest, *source;
   const float *weights;
   uint32_t tokens, slots, rows, vectors, unused_blocks;
+  FastDiv by_slots;
   int lx;
 };
 
@@ -150,51 +151,56 @@ __global__ void __launch_bounds__(kRowThreads) combine_kernel(Route p) {
   out.store_cs(static_cast<T *>(p.out) + token * p.out_pitch + (uint64_t)c * V);
 }
 
-// A block takes a token: its dout row meets each of the token's rows of y.
+// (1 << lx) lanes, a warp at most, take an entry: the token's row of dout meets the
+// entry's row of y.  The entries of a token are neighbours, so that its row comes from
+// L2 after the first.  (A block a token, slot after slot, with block-wide sums: 210 us
+// instead of 186 for 16384 tokens x 8 slots x 2048 bf16.)
 template <typename T, int V>
 __global__ void __launch_bounds__(kRowThreads) combine_grad_kernel(Route p) {
-  __shared__ float part[kRowThreads / 32];
   pdl_trigger_at_entry();
   pdl_wait();
   pdl_launch_dependents();
   if (blockIdx.x < p.unused_blocks)
     return zero_unused<(int)sizeof(T) * V>(p, p.out_pitch * sizeof(T));
-  const uint32_t token = blockIdx.x - p.unused_blocks;
-  const T *dout = static_cast<const T *>(p.dout) + token * p.dout_pitch;
-  for (uint32_t j = 0; j < p.slots; ++j) {
-    const int32_t row = p.dest[(uint64_t)token * p.slots + j];
-    const bool kept = row >= 0 && (uint32_t)row < p.rows;
-    float dot = 0.0f;
-    if (kept) {
-      const float w = p.weights[token * p.w_pitch + j];
-      const T *y = static_cast<const T *>(p.in) + row * p.in_pitch;
-      T *dy = static_cast<T *>(p.out) + row * p.out_pitch;
-      for (uint32_t c = threadIdx.x; c < p.vectors; c += blockDim.x) {
-        Vec<T, V> g, in, out;
-        g.load(dout + (uint64_t)c * V);
-        in.load(y + (uint64_t)c * V);
-        float f[V];
+  const uint32_t entry =
+      (blockIdx.x - p.unused_blocks) * (kRowThreads >> p.lx) + (threadIdx.x >> p.lx);
+  const uint32_t lanes = 1u << p.lx, lane = threadIdx.x & (lanes - 1);
+  const uint32_t token = p.by_slots.div(entry), slot = entry - token * p.slots;
+  const bool there = token < p.tokens;
+  const int32_t row = there ? p.dest[entry] : -1;
+  float dot = 0.0f;
+  if (row >= 0 && (uint32_t)row < p.rows) {
+    const float w = p.weights[token * p.w_pitch + slot];
+    const T *dout = static_cast<const T *>(p.dout) + token * p.dout_pitch;
+    const T *y = static_cast<const T *>(p.in) + row * p.in_pitch;
+    T *dy = static_cast<T *>(p.out) + row * p.out_pitch;
+    constexpr int U = 4;
+    for (uint32_t c0 = lane; c0 < p.vectors; c0 += U * lanes) {
+      Vec<T, V> g[U], in[U];
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float d = g.get(i);
-          dot = fmaf(d, in.get(i), dot);
-          f[i] = d * w;
+      for (int u = 0; u < U; ++u)
+        if (c0 + u * lanes < p.vectors) {
+          in[u].load(y + (uint64_t)(c0 + u * lanes) * V);
+          g[u].load(dout + (uint64_t)(c0 + u * lanes) * V);
         }
-        out.put(f);
-        out.store_cs(dy + (uint64_t)c * V);
-      }
-    }
 #pragma unroll
-    for (int o = 16; o; o /= 2) dot += __shfl_xor_sync(~0u, dot, o);
-    if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = dot;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      float all = 0.0f;
-      for (uint32_t w = 0; w < blockDim.x / 32; ++w) all += part[w];
-      p.dweights[token * p.dw_pitch + j] = all;
+      for (int u = 0; u < U; ++u)
+        if (c0 + u * lanes < p.vectors) {
+          float f[V];
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            const float d = g[u].get(i);
+            dot = fmaf(d, in[u].get(i), dot);
+            f[i] = d * w;
+          }
+          Vec<T, V> out;
+          out.put(f);
+          out.store_cs(dy + (uint64_t)(c0 + u * lanes) * V);
+        }
     }
-    __syncthreads();
   }
+  for (uint32_t o = lanes / 2; o; o /= 2) dot += __shfl_xor_sync(~0u, dot, o);
+  if (lane == 0 && there) p.dweights[token * p.dw_pitch + slot] = dot;
 }
 
 int check_route(const int32_t *dest, int64_t tokens, int64_t slots, const int32_t *source,
@@ -447,16 +453,21 @@ int dcopy_expert_combine_grad(const DcopyMatrix *dy, const DcopyMatrix *dweights
   p.slots = (uint32_t)slots;
   p.rows = (uint32_t)dy->rows;
   p.unused_blocks = unused_blocks(source, dy->rows);
-  const uint32_t blocks = p.tokens + p.unused_blocks;
-  if (blocks == 0) return DCOPY_OK;
+  p.by_slots = FastDiv((uint32_t)std::max<int64_t>(1, slots));
+  const uint64_t entries = (uint64_t)p.tokens * p.slots;
   return with_float(dy->type, [&](auto t) {
     using T = typename decltype(t)::type;
     const int v = std::min(std::min(vector_width(dy), vector_width(dout)), vector_width(y));
     return with_vector<sizeof(T)>(v, [&](auto vw) {
       constexpr int V = decltype(vw)::value;
       p.vectors = (uint32_t)(dy->cols / V);
-      return launch_grid(combine_grad_kernel<T, V>, dim3(blocks), dim3(kRowThreads), 0, stream,
-                         "combine_grad_kernel", p);
+      p.lx = 0;
+      while (p.lx < 5 && (1u << p.lx) < p.vectors) ++p.lx;
+      const uint64_t per_block = kRowThreads >> p.lx;
+      const uint64_t blocks = p.unused_blocks + (entries + per_block - 1) / per_block;
+      if (blocks == 0) return (int)DCOPY_OK;
+      return launch(combine_grad_kernel<T, V>, (unsigned)blocks, dim3(kRowThreads), 0, stream,
+                    "combine_grad_kernel", p);
     });
   });
   DCOPY_API_END
