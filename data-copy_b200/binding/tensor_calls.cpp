@@ -1,0 +1,419 @@
+// dcopy._tensor_calls: the model operators' C ABI called on torch tensors.
+//
+// Reads rows, pitch and type of each tensor, takes torch's current stream of the
+// tensors' device (made current for the call) unless one is given, and a workspace
+// from torch's allocator unless one is given.  The same in Python took 5 us a call
+// besides the launch, more than the smallest operators run on the GPU; here it is
+// under 1 us.  The functions of libdcopy.so are handed over by address (bind), so
+// that one copy of the library is loaded.
+#include <Python.h>
+
+#include <ATen/core/Tensor.h>
+#include <ATen/ops/empty.h>
+#include <c10/cuda/CUDACachingAllocator.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/python_variable.h>
+
+#include <optional>
+#include <string>
+
+#include "dcopy/dcopy.h"
+
+namespace {
+
+#define DCOPY_CALLS(X)                                                                     \
+  X(dcopy_last_error_message)                                                              \
+  X(dcopy_embedding_lookup) X(dcopy_embedding_grad) X(dcopy_embedding_grad_workspace)      \
+  X(dcopy_expert_sort) X(dcopy_expert_sort_workspace) X(dcopy_expert_dispatch)             \
+  X(dcopy_expert_combine) X(dcopy_expert_combine_grad)                                     \
+  X(dcopy_grad_sum_squares) X(dcopy_grad_clip) X(dcopy_clip_grad_norm)
+
+struct Library {
+#define X(name) decltype(&::name) name = nullptr;
+  DCOPY_CALLS(X)
+#undef X
+} lib;
+PyObject *error_class = nullptr;  // dcopy.DcopyError
+
+// A Python exception is set; carried to the entry point as a C++ one.
+struct Raised {};
+
+[[noreturn]] void value_error(const char *name, const std::string &what) {
+  PyErr_Format(PyExc_ValueError, "%s: %s", name, what.c_str());
+  throw Raised{};
+}
+
+[[noreturn]] void dcopy_error(int code, const std::string &message, const char *func) {
+  PyObject *e = PyObject_CallFunction(error_class, "iss", code, message.c_str(), func);
+  if (e) {
+    PyErr_SetObject(error_class, e);
+    Py_DECREF(e);
+  }
+  throw Raised{};
+}
+
+int32_t type_code(at::ScalarType t) {  // the GE DataType; -1, which the library refuses
+  switch (t) {
+    case at::kFloat: return 0;
+    case at::kHalf: return 1;
+    case at::kChar: return 2;
+    case at::kInt: return 3;
+    case at::kByte: case at::kFloat8_e4m3fn: case at::kFloat8_e5m2: return 4;
+    case at::kLong: return 9;
+    case at::kBFloat16: return 27;
+    default: return -1;
+  }
+}
+
+const at::Tensor &unpack(PyObject *o, const char *name) {
+  if (!THPVariable_Check(o)) value_error(name, "expected a tensor");
+  return THPVariable_Unpack(o);
+}
+
+// A tensor as rows of its last dimension; the other dimensions must step evenly.
+DcopyMatrix layout(const at::Tensor &t, const char *name) {
+  DcopyMatrix m{};
+  const auto shape = t.sizes(), stride = t.strides();
+  const int64_t d = (int64_t)shape.size();
+  int64_t unit = 1;
+  if (d < 2) {
+    m.rows = 1;
+    m.cols = t.numel();
+    unit = d ? stride[0] : 1;
+    if (unit != 1) {  // a strided vector: rows of one element
+      m.rows = m.cols, m.cols = 1, m.pitch = unit, unit = 1;
+      if (m.pitch < 1 && m.rows > 1) value_error(name, "elements repeat");
+    }
+  } else {
+    m.cols = shape[d - 1];
+    unit = stride[d - 1];
+    m.pitch = stride[d - 2];
+    m.rows = 1;
+    for (int64_t k = d - 2; k >= 0; --k) {
+      if (shape[k] > 1) {
+        if (m.rows == 1) m.pitch = stride[k];
+        else if (stride[k] != m.rows * m.pitch) value_error(name, "rows do not lie at one pitch");
+      }
+      m.rows *= shape[k];
+    }
+  }
+  if (unit != 1 && m.cols > 1) value_error(name, "the last dimension must be dense");
+  m.data = const_cast<void *>(t.const_data_ptr());
+  m.type = type_code(t.scalar_type());
+  return m;
+}
+
+int64_t as_int(PyObject *o) {
+  const long long v = PyLong_AsLongLong(o);
+  if (v == -1 && PyErr_Occurred()) throw Raised{};
+  return v;
+}
+double as_double(PyObject *o) {
+  const double v = PyFloat_AsDouble(o);
+  if (v == -1.0 && PyErr_Occurred()) throw Raised{};
+  return v;
+}
+
+// One call: its device, which all its tensors share, and its stream.
+class Call {
+ public:
+  Call(const char *func, PyObject *stream) : func_(func), given_(stream) {}
+
+  const at::Tensor &tensor(PyObject *o, const char *name) {
+    const at::Tensor &t = unpack(o, name);
+    if (!t.is_cuda()) value_error(name, "expected a CUDA tensor");
+    if (device_ < 0) device_ = t.get_device();
+    else if (t.get_device() != device_) value_error(name, "tensors are on different devices");
+    return t;
+  }
+  DcopyMatrix matrix(PyObject *o, const char *name) { return layout(tensor(o, name), name); }
+  // A dense tensor of one type, or None (nullptr).
+  void *vector(PyObject *o, const char *name, at::ScalarType type, int64_t *count = nullptr) {
+    if (o == Py_None) return nullptr;
+    const at::Tensor &t = tensor(o, name);
+    if (!t.is_contiguous() || t.scalar_type() != type)
+      value_error(name, std::string("expected a contiguous CUDA tensor of type ") +
+                            c10::toString(type));
+    if (count) *count = t.numel();
+    return const_cast<void *>(t.const_data_ptr());
+  }
+  void on_device(int64_t device) { device_ = device; }
+
+  // Fixes device and stream; after the tensors were read.
+  dcopy_stream_t stream() {
+    guard_.emplace((c10::DeviceIndex)device_);
+    if (given_ == Py_None)
+      return reinterpret_cast<dcopy_stream_t>(
+          c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device_).stream());
+    PyObject *value = PyLong_Check(given_) ? Py_NewRef(given_)
+                                           : PyObject_GetAttrString(given_, "cuda_stream");
+    if (!value) throw Raised{};
+    const unsigned long long raw = PyLong_AsUnsignedLongLong(value);
+    Py_DECREF(value);
+    if (PyErr_Occurred()) throw Raised{};
+    return reinterpret_cast<dcopy_stream_t>((uintptr_t)raw);
+  }
+  // The given workspace, or one from the allocator that is kept until `s` is done.
+  void *workspace(PyObject *o, uint64_t need, dcopy_stream_t s, uint64_t *bytes) {
+    if (o != Py_None) {
+      const at::Tensor &t = tensor(o, "workspace");
+      if (!t.is_contiguous()) value_error("workspace", "expected a contiguous tensor");
+      *bytes = t.nbytes();
+      return const_cast<void *>(t.const_data_ptr());
+    }
+    scratch_ = at::empty({(int64_t)need}, at::TensorOptions().dtype(at::kByte).device(
+                                              at::Device(at::kCUDA, (c10::DeviceIndex)device_)));
+    const auto ext = c10::cuda::getStreamFromExternal(reinterpret_cast<cudaStream_t>(s),
+                                                      (c10::DeviceIndex)device_);
+    if (given_ != Py_None)
+      c10::cuda::CUDACachingAllocator::recordStream(scratch_.storage().data_ptr(), ext);
+    *bytes = need;
+    return scratch_.mutable_data_ptr();
+  }
+  void check(int rc) {
+    if (rc) dcopy_error(rc, lib.dcopy_last_error_message(), func_);
+  }
+  const char *func() const { return func_; }
+
+ private:
+  const char *func_;
+  PyObject *given_;
+  int64_t device_ = -1;
+  std::optional<c10::cuda::CUDAGuard> guard_;
+  at::Tensor scratch_;
+};
+
+// Runs a call's body; C++ exceptions end here.
+template <typename F>
+PyObject *run(const char *func, PyObject *const *a, Py_ssize_t n, Py_ssize_t want, F &&body) {
+  if (n != want) {
+    PyErr_Format(PyExc_TypeError, "%s takes %zd arguments", func, want);
+    return nullptr;
+  }
+  if (!lib.dcopy_last_error_message) {
+    PyErr_SetString(PyExc_RuntimeError, "dcopy._tensor_calls is not bound to the library");
+    return nullptr;
+  }
+  try {
+    Call call(func, a[n - 1]);  // the stream comes last
+    body(call);
+    Py_RETURN_NONE;
+  } catch (const Raised &) {
+  } catch (const std::exception &e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+  } catch (...) {
+    PyErr_SetString(PyExc_RuntimeError, "internal exception");
+  }
+  return nullptr;
+}
+
+// Without the interpreter's lock: a launch may wait for room in the stream's queue.
+template <typename F>
+int unlocked(F &&f) {
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = f();
+  Py_END_ALLOW_THREADS
+  return rc;
+}
+
+PyObject *embedding_lookup(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  return run("dcopy_embedding_lookup", a, n, 6, [&](Call &c) {
+    const DcopyMatrix out = c.matrix(a[0], "out"), table = c.matrix(a[1], "table"),
+                      ids = c.matrix(a[2], "ids");
+    const float scale = (float)as_double(a[3]);
+    const int64_t first = as_int(a[4]);
+    dcopy_stream_t s = c.stream();
+    c.check(unlocked([&] { return lib.dcopy_embedding_lookup(&out, &table, &ids, first, scale, s); }));
+  });
+}
+
+PyObject *embedding_grad(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  return run("dcopy_embedding_grad", a, n, 8, [&](Call &c) {
+    const DcopyMatrix grad = c.matrix(a[0], "grad"), dout = c.matrix(a[1], "dout"),
+                      ids = c.matrix(a[2], "ids");
+    const float scale = (float)as_double(a[3]);
+    const int64_t first = as_int(a[4]);
+    const int accumulate = PyObject_IsTrue(a[5]);
+    dcopy_stream_t s = c.stream();
+    uint64_t need = 0, bytes = 0;
+    if (a[6] == Py_None)
+      c.check(lib.dcopy_embedding_grad_workspace(ids.rows * ids.cols, grad.rows, grad.cols, &need));
+    void *space = c.workspace(a[6], need, s, &bytes);
+    c.check(unlocked([&] {
+      return lib.dcopy_embedding_grad(&grad, &dout, &ids, first, scale, accumulate, space, bytes, s);
+    }));
+  });
+}
+
+PyObject *expert_sort(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  return run("dcopy_expert_sort", a, n, 7, [&](Call &c) {
+    int64_t entries = 0, rows = 0, ends = 0;
+    auto *dest = (int32_t *)c.vector(a[0], "dest", at::kInt, &entries);
+    auto *source = (int32_t *)c.vector(a[1], "source", at::kInt, &rows);
+    auto *offsets = (int32_t *)c.vector(a[2], "offsets", at::kInt, &ends);
+    const DcopyMatrix ids = c.matrix(a[3], "expert_ids");
+    if (entries != ids.rows * ids.cols)
+      dcopy_error(DCOPY_ERR_SHAPE_INVALID, "dest has " + std::to_string(entries) + " values for " +
+                  std::to_string(ids.rows * ids.cols) + " choices", c.func());
+    const int32_t align = (int32_t)as_int(a[4]), experts = (int32_t)(ends - 1);
+    dcopy_stream_t s = c.stream();
+    uint64_t need = 0, bytes = 0;
+    if (a[5] == Py_None) c.check(lib.dcopy_expert_sort_workspace(entries, experts, &need));
+    void *space = c.workspace(a[5], need, s, &bytes);
+    c.check(unlocked([&] {
+      return lib.dcopy_expert_sort(dest, source, rows, offsets, &ids, experts, align, space, bytes, s);
+    }));
+  });
+}
+
+// dest and source of a routing of `tokens` tokens into `rows` rows.
+struct Routing {
+  const int32_t *dest, *source;
+  int64_t slots;
+};
+Routing routing(Call &c, PyObject *dest, PyObject *source, int64_t tokens, int64_t rows) {
+  Routing r{};
+  int64_t n = 0, held = rows;
+  r.dest = (const int32_t *)c.vector(dest, "dest", at::kInt, &n);
+  r.source = (const int32_t *)c.vector(source, "source", at::kInt, &held);
+  if (dest != Py_None && unpack(dest, "dest").dim() > 1) r.slots = unpack(dest, "dest").size(-1);
+  else r.slots = tokens ? n / tokens : 0;
+  if (r.slots * tokens != n)
+    dcopy_error(DCOPY_ERR_SHAPE_INVALID, "dest has " + std::to_string(n) + " values for " +
+                std::to_string(tokens) + " tokens", c.func());
+  if (held != rows)
+    dcopy_error(DCOPY_ERR_SHAPE_INVALID, "source has " + std::to_string(held) + " values for " +
+                std::to_string(rows) + " rows", c.func());
+  return r;
+}
+
+PyObject *expert_dispatch(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  return run("dcopy_expert_dispatch", a, n, 6, [&](Call &c) {
+    const DcopyMatrix out = c.matrix(a[0], "out"), x = c.matrix(a[1], "x");
+    const Routing r = routing(c, a[2], a[3], x.rows, out.rows);
+    DcopyMatrix weights{};
+    const bool weighted = a[4] != Py_None;
+    if (weighted) weights = c.matrix(a[4], "weights");
+    dcopy_stream_t s = c.stream();
+    c.check(unlocked([&] {
+      return lib.dcopy_expert_dispatch(&out, &x, r.dest, r.slots, r.source,
+                                       weighted ? &weights : nullptr, s);
+    }));
+  });
+}
+
+PyObject *expert_combine(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  return run("dcopy_expert_combine", a, n, 5, [&](Call &c) {
+    const DcopyMatrix out = c.matrix(a[0], "out"), y = c.matrix(a[1], "y");
+    const Routing r = routing(c, a[2], Py_None, out.rows, y.rows);
+    DcopyMatrix weights{};
+    const bool weighted = a[3] != Py_None;
+    if (weighted) weights = c.matrix(a[3], "weights");
+    dcopy_stream_t s = c.stream();
+    c.check(unlocked([&] {
+      return lib.dcopy_expert_combine(&out, &y, r.dest, r.slots, weighted ? &weights : nullptr, s);
+    }));
+  });
+}
+
+PyObject *expert_combine_grad(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  return run("dcopy_expert_combine_grad", a, n, 8, [&](Call &c) {
+    const DcopyMatrix dy = c.matrix(a[0], "dy"), dw = c.matrix(a[1], "dweights"),
+                      dout = c.matrix(a[2], "dout"), y = c.matrix(a[3], "y"),
+                      weights = c.matrix(a[5], "weights");
+    const Routing r = routing(c, a[4], a[6], dout.rows, dy.rows);
+    dcopy_stream_t s = c.stream();
+    c.check(unlocked([&] {
+      return lib.dcopy_expert_combine_grad(&dy, &dw, &dout, &y, r.dest, r.slots, r.source, &weights,
+                                           s);
+    }));
+  });
+}
+
+// (address of the DcopyGradList, device, ...)
+const DcopyGradList *grad_list(Call &c, PyObject *address, PyObject *device) {
+  c.on_device(as_int(device));
+  return reinterpret_cast<const DcopyGradList *>((uintptr_t)as_int(address));
+}
+
+PyObject *grad_sum_squares(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  return run("dcopy_grad_sum_squares", a, n, 4, [&](Call &c) {
+    const DcopyGradList *list = grad_list(c, a[0], a[1]);
+    auto *total = (double *)c.vector(a[2], "total", at::kDouble);
+    dcopy_stream_t s = c.stream();
+    c.check(unlocked([&] { return lib.dcopy_grad_sum_squares(list, total, s); }));
+  });
+}
+
+PyObject *grad_clip(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  return run("dcopy_grad_clip", a, n, 7, [&](Call &c) {
+    const DcopyGradList *list = grad_list(c, a[0], a[1]);
+    auto *total = (const double *)c.vector(a[2], "total", at::kDouble);
+    const float max_norm = (float)as_double(a[3]), eps = (float)as_double(a[4]);
+    auto *norm = (float *)c.vector(a[5], "norm", at::kFloat);
+    dcopy_stream_t s = c.stream();
+    c.check(unlocked([&] { return lib.dcopy_grad_clip(list, total, max_norm, eps, norm, s); }));
+  });
+}
+
+PyObject *clip_grad_norm(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  return run("dcopy_clip_grad_norm", a, n, 6, [&](Call &c) {
+    const DcopyGradList *list = grad_list(c, a[0], a[1]);
+    const float max_norm = (float)as_double(a[2]), eps = (float)as_double(a[3]);
+    auto *norm = (float *)c.vector(a[4], "norm", at::kFloat);
+    dcopy_stream_t s = c.stream();
+    c.check(unlocked([&] { return lib.dcopy_clip_grad_norm(list, max_norm, eps, norm, s); }));
+  });
+}
+
+// layout(tensor) -> (rows, cols, pitch, type): how a call sees a tensor, on any device.
+PyObject *layout_of(PyObject *, PyObject *o) {
+  try {
+    const DcopyMatrix m = layout(unpack(o, "tensor"), "tensor");
+    return Py_BuildValue("LLLi", (long long)m.rows, (long long)m.cols, (long long)m.pitch, m.type);
+  } catch (const Raised &) {
+  } catch (const std::exception &e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+  }
+  return nullptr;
+}
+
+// bind({name: address}, DcopyError)
+PyObject *bind(PyObject *, PyObject *args) {
+  PyObject *addresses = nullptr, *error = nullptr;
+  if (!PyArg_ParseTuple(args, "O!O", &PyDict_Type, &addresses, &error)) return nullptr;
+  Library found;
+#define X(name)                                                                 \
+  {                                                                             \
+    PyObject *v = PyDict_GetItemString(addresses, #name);                       \
+    void *p = v ? PyLong_AsVoidPtr(v) : nullptr;                                \
+    if (!p) {                                                                   \
+      if (!PyErr_Occurred()) PyErr_SetString(PyExc_KeyError, #name);            \
+      return nullptr;                                                           \
+    }                                                                           \
+    found.name = reinterpret_cast<decltype(&::name)>(p);                        \
+  }
+  DCOPY_CALLS(X)
+#undef X
+  lib = found;
+  Py_XSETREF(error_class, Py_NewRef(error));
+  Py_RETURN_NONE;
+}
+
+#define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(name)), METH_FASTCALL, nullptr}
+PyMethodDef methods[] = {
+    FAST(embedding_lookup), FAST(embedding_grad), FAST(expert_sort), FAST(expert_dispatch),
+    FAST(expert_combine), FAST(expert_combine_grad), FAST(grad_sum_squares), FAST(grad_clip),
+    FAST(clip_grad_norm),
+    {"layout", layout_of, METH_O, nullptr},
+    {"bind", bind, METH_VARARGS, nullptr},
+    {nullptr, nullptr, 0, nullptr}};
+
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensor_calls", nullptr, -1, methods,
+                      nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__tensor_calls(void) { return PyModule_Create(&module); }

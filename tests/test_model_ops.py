@@ -82,22 +82,12 @@ def test_python_refuses_host_tensors(dcopy):
         dcopy.GradList([])
 
 
-def test_matrix_of_a_tensor(dcopy, monkeypatch):
-    """Rows and pitch that the binding reads from a tensor's shape and strides."""
+def test_layout_of_a_tensor(dcopy):
+    """Rows, columns, pitch and type that a call reads from a tensor's shape and strides."""
     from dcopy import model_ops
 
-    class Fake:  # a tensor's layout as if it lay in device memory
-        is_cuda = True
-
-        def __init__(self, t):
-            self.t = t
-
-        def __getattr__(self, name):
-            return getattr(self.t, name)
-
     def read(t):
-        m = model_ops._matrix(Fake(t), "t")
-        return m.rows, m.cols, m.pitch, m.type
+        return model_ops._calls.layout(t)
 
     x = torch.zeros(6, 10, 16)
     assert read(x) == (60, 16, 16, 0)
@@ -109,10 +99,14 @@ def test_matrix_of_a_tensor(dcopy, monkeypatch):
     assert read(torch.zeros(12, dtype=torch.int64)) == (1, 12, 0, 9)
     assert read(torch.zeros(12, dtype=torch.int32)[::3]) == (4, 1, 3, 3)
     assert read(torch.zeros(9, 1)) == (9, 1, 1, 0)
+    assert read(torch.zeros(3, 4, dtype=torch.float64)) == (3, 4, 4, -1)
+    for bad in (x[:, :5],                       # two row pitches
+                torch.zeros(4, 6).t(),          # columns that are not dense
+                torch.zeros(1).expand(5)):      # one element for all
+        with pytest.raises(ValueError):
+            read(bad)
     with pytest.raises(ValueError):
-        read(x[:, :5])  # two row pitches
-    with pytest.raises(ValueError):
-        read(torch.zeros(4, 6).t())  # columns that are not dense
+        read([1, 2])
 
 
 def test_records_match_the_c_abi(dcopy, tmp_path, monkeypatch):
