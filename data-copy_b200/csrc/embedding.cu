@@ -30,12 +30,12 @@ struct Lookup {
   const void *table;
   int64_t out_pitch, table_pitch;
   KeySource ids;
-  uint32_t vectors;
+  uint32_t width, vectors;
   int lx;
   float scale;
 };
 
-template <typename TIn, typename TOut, int V, int U>
+template <typename TIn, typename TOut, int V, bool kShift, int U>
 __global__ void __launch_bounds__(kRowThreads) lookup_kernel(Lookup p) {
   pdl_trigger_at_entry();
   pdl_wait();
@@ -43,27 +43,28 @@ __global__ void __launch_bounds__(kRowThreads) lookup_kernel(Lookup p) {
   const uint32_t row = blockIdx.x * (kRowThreads >> p.lx) + (threadIdx.x >> p.lx);
   if (row >= p.ids.n) return;
   const uint32_t step = 1u << p.lx;
-  const uint32_t c0 = (blockIdx.y * U << p.lx) + (threadIdx.x & (step - 1));
+  const uint32_t q = (blockIdx.y * U << p.lx) + (threadIdx.x & (step - 1));
   const int64_t id = read_id(p.ids, row);
   const bool known = id >= 0 && id < (int64_t)p.ids.keys;
   const TIn *src = static_cast<const TIn *>(p.table) + (known ? id * p.table_pitch : 0);
   TOut *dst = static_cast<TOut *>(p.out) + row * p.out_pitch;
+  const int32_t lead = row_lead<TOut, V, kShift>(dst);
   Vec<TIn, V> in[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const uint32_t c = c0 + u * step;
-    if (known && c < p.vectors) in[u].load(src + (uint64_t)c * V);
+    const int32_t c = (int32_t)((q + u * step) * V) - lead;
+    if (known && c < (int32_t)p.width) load_columns<TIn, V, kShift>(in[u], src, c, p.width);
     else in[u].zero();
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const uint32_t c = c0 + u * step;
+    const int32_t c = (int32_t)((q + u * step) * V) - lead;
     float f[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) f[i] = known ? in[u].get(i) * p.scale : 0.0f;
     Vec<TOut, V> out;
     out.put(f);
-    if (c < p.vectors) out.store_cs(dst + (uint64_t)c * V);
+    if (c < (int32_t)p.width) store_columns<TOut, V, kShift>(out, dst, c, p.width);
   }
 }
 
@@ -306,13 +307,21 @@ int dcopy_embedding_lookup(const DcopyMatrix *out, const DcopyMatrix *table,
     return with_float(out->type, [&](auto tout) {
       using TIn = typename decltype(tin)::type;
       using TOut = typename decltype(tout)::type;
-      return with_vector<std::max(sizeof(TIn), sizeof(TOut))>(std::min(vector_width(out), vector_width(table)), [&](auto vw) {
-        constexpr int V = decltype(vw)::value;
-        p.vectors = (uint32_t)(out->cols / V);
-        const bool many = (uint64_t)p.ids.n * p.vectors >= (uint64_t)sm_count() * 2048 * 4;
-        const RowSplit split = split_rows(p.ids.n, p.vectors, many ? 4 : 1);
-        p.lx = split.lx;
-        auto k = many ? lookup_kernel<TIn, TOut, V, 4> : lookup_kernel<TIn, TOut, V, 1>;
+      // Shifted below 8-byte vectors (16384 rows of 1025 bf16: 25 us against 60 in single
+      // elements; of 1025 fp32: 21 against 33).
+      constexpr int kBytes = std::max(sizeof(TIn), sizeof(TOut));
+      constexpr int kFull = 16 / kBytes, kLeast = 8 / kBytes;
+      const Cut cut = cut_rows(kFull, kLeast, out, table);
+      p.width = (uint32_t)out->cols;
+      p.vectors = vectors_of(out->cols, cut);
+      // Four vectors a thread (32 Ki rows of 8 KB: 62 us, 75 with one), one where the
+      // grid is small.
+      const bool many = (uint64_t)p.ids.n * p.vectors >= (uint64_t)sm_count() * 2048 * 4;
+      const RowSplit split = split_rows(p.ids.n, p.vectors, many ? 4 : 1);
+      p.lx = split.lx;
+      return with_cut<kFull, kLeast>(cut, [&](auto v, auto shift) {
+        auto k = many ? lookup_kernel<TIn, TOut, v(), shift(), 4>
+                      : lookup_kernel<TIn, TOut, v(), shift(), 1>;
         return launch_grid(k, split.grid, dim3(kRowThreads), 0, stream, "lookup_kernel", p);
       });
     });
@@ -389,9 +398,12 @@ int dcopy_embedding_grad(const DcopyMatrix *grad, const DcopyMatrix *dout, const
     return with_float(grad->type, [&](auto tout) {
       using TIn = typename decltype(tin)::type;
       using TOut = typename decltype(tout)::type;
-      return with_vector<std::max(sizeof(TIn), sizeof(TOut))>(std::min(vector_width(dout), vector_width(grad)), [&](auto vw) {
-        constexpr int V = decltype(vw)::value;
-        p.vectors = (uint32_t)(grad->cols / V);
+      // Never shifted: 16384 tokens of 1026 bf16 take 83 us in 4-byte vectors, 107 shifted.
+      constexpr int kFull = 16 / std::max(sizeof(TIn), sizeof(TOut));
+      const Cut cut = cut_rows(kFull, 1, grad, dout);
+      p.vectors = vectors_of(grad->cols, cut);
+      return with_cut<kFull, 1>(cut, [&](auto v, auto) {
+        constexpr int V = v();
         const RowSplit split = split_rows(p.pieces, p.vectors, 1, kMaxPieces);
         p.lx = split.lx;
         auto sum = accumulate ? piece_sum_kernel<TIn, TOut, V, true>

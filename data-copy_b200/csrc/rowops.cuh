@@ -11,6 +11,7 @@
 #include <algorithm>
 
 #include "common.cuh"
+#include "shift.cuh"
 
 namespace dcopy {
 
@@ -236,26 +237,127 @@ inline RowSplit split_rows(uint64_t rows, uint64_t vectors, int u, int most_rows
   return s;
 }
 
-// Calls f with a value of type std::integral_constant<int, V> for the vector width v
-// (as vector_width gives it) of elements of at most kBytes bytes.
-template <int kBytes, typename F>
+// How the rows of an operator's matrices are cut into vectors of V elements.  Where every
+// row starts on a vector and is whole vectors, they are accessed as they lie.  Rows for
+// which only vectors of few bytes would do are cut at the 16-byte granules of the row that
+// is written, and read by pairs of aligned blocks that are shifted together (kShift); the
+// operators that gain by it say from which size on.
+struct Cut {
+  int v;
+  bool shift;
+};
+
+// full: elements of 16 bytes of the widest type; least: below so many, shift.
+template <typename... M>
+Cut cut_rows(int full, int least, const M *...m) {
+  const int v = std::min({full, vector_width(m)...});
+  return v >= least ? Cut{v, false} : Cut{full, true};
+}
+
+// Vectors that cover a row: with shifted cuts one more at each end may hold part of it.
+inline uint32_t vectors_of(int64_t width, Cut c) {
+  return (uint32_t)(c.shift ? (width + 2 * c.v - 2) / c.v : width / c.v);
+}
+
+// Calls f(V, kShift) as compile-time constants; kFull and kLeast as in cut_rows.
+template <int kV, int kLeast, typename F>
 int with_vector(int v, F &&f) {
-  if constexpr (kBytes <= 2)
-    if (v == 8) return f(std::integral_constant<int, 8>{});
-  if (v == 4) return f(std::integral_constant<int, 4>{});
-  if (v == 2) return f(std::integral_constant<int, 2>{});
-  return f(std::integral_constant<int, 1>{});
+  if constexpr (kV / 2 >= kLeast && kV > 1)
+    if (v < kV) return with_vector<kV / 2, kLeast>(v, f);
+  return f(std::integral_constant<int, kV>{}, std::false_type{});
+}
+template <int kFull, int kLeast, typename F>
+int with_cut(Cut c, F &&f) {
+  if constexpr (kLeast > 1)
+    if (c.shift) return f(std::integral_constant<int, kFull>{}, std::true_type{});
+  return with_vector<kFull, kLeast>(c.v, f);
+}
+
+// 16 or 8 bytes (N) from address a, those of them that lie in [begin, end); the others
+// are unspecified.  A block is only loaded when it holds a byte of the range, so every
+// load stays inside the page of a byte that the caller owns.
+template <int N>
+__device__ __forceinline__ Words<N> load_shifted(uintptr_t a, uintptr_t begin, uintptr_t end) {
+  const uint32_t s = (uint32_t)(a & (N - 1));
+  const uintptr_t b = a - s;
+  const bool first = b < end && b + N > begin, second = s && b + N < end && b + 2 * N > begin;
+  Words<N> out;
+  if constexpr (N == 16) {
+    uint4 x = make_uint4(0, 0, 0, 0), y = x;
+    if (first) x = __ldg(reinterpret_cast<const uint4 *>(b));
+    if (second) y = __ldg(reinterpret_cast<const uint4 *>(b) + 1);
+    x = shift_pair(x, y, s);
+    out.w[0] = x.x, out.w[1] = x.y, out.w[2] = x.z, out.w[3] = x.w;
+  } else {
+    uint2 x = make_uint2(0, 0), y = x;
+    if (first) x = __ldg(reinterpret_cast<const uint2 *>(b));
+    if (second) y = __ldg(reinterpret_cast<const uint2 *>(b) + 1);
+    uint32_t w0 = x.x, w1 = x.y, w2 = y.x;
+    if (s & 4) w0 = w1, w1 = w2, w2 = y.y;
+    const uint32_t r = (s & 3) * 8;
+    out.w[0] = __funnelshift_r(w0, w1, r), out.w[1] = __funnelshift_r(w1, w2, r);
+  }
+  return out;
+}
+
+// V elements of a row from column c on.  With kShift c may be any column from 1 - V on;
+// elements outside the row are unspecified.
+template <typename T, int V, bool kShift>
+__device__ __forceinline__ void load_columns(Vec<T, V> &v, const T *row, int32_t c,
+                                             uint32_t width) {
+  if constexpr (kShift) {
+    const uintptr_t begin = reinterpret_cast<uintptr_t>(row);
+    static_cast<Words<(int)sizeof(T) * V> &>(v) = load_shifted<(int)sizeof(T) * V>(
+        begin + (int64_t)c * (int)sizeof(T), begin, begin + (uint64_t)width * sizeof(T));
+  } else {
+    v.load(row + c);
+  }
+}
+
+// Columns by which a row that is written precedes its first granule: vector q of the
+// row holds the columns from q * V - lead on.
+template <typename T, int V, bool kShift>
+__device__ __forceinline__ int32_t row_lead(const T *row) {
+  if constexpr (!kShift) return 0;
+  return (int32_t)(reinterpret_cast<uintptr_t>(row) % (V * sizeof(T)) / sizeof(T));
+}
+
+// Whether all of a vector lies in the row.
+template <int V, bool kShift>
+__device__ __forceinline__ bool whole(int32_t c, uint32_t width) {
+  return !kShift || (c >= 0 && c + V <= (int32_t)width);
+}
+
+template <typename T, int V, bool kShift, bool kStream = true>
+__device__ __forceinline__ void store_columns(const Vec<T, V> &v, T *row, int32_t c,
+                                              uint32_t width) {
+  if (whole<V, kShift>(c, width)) {
+    if constexpr (kStream) v.store_cs(row + c);
+    else v.store(row + c);
+  } else if constexpr (kShift) {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (c + i >= 0 && c + i < (int32_t)width) {
+        Words<(int)sizeof(T)> one;
+        one.w[0] = sizeof(T) == 4 ? v.w[i] : v.w[i / 2] >> 16 * (i & 1);
+        one.store(row + c + i);
+      }
+  }
 }
 
 // Zeroes `bytes` bytes by the threads `t` of `threads`: 16-byte granules, bytes at the
 // ends.
+template <bool kStream = false>
 __device__ __forceinline__ void zero_bytes(uint8_t *at, uint64_t bytes, uint32_t t,
                                            uint32_t threads) {
   const uint64_t head = min((uint64_t)(-(uintptr_t)at & 15), bytes);
   const uint64_t units = (bytes - head) / 16, tail = bytes - head - units * 16;
   uint4 *dst = reinterpret_cast<uint4 *>(at + head);
 #pragma unroll 4
-  for (uint64_t u = t; u < units; u += threads) dst[u] = make_uint4(0, 0, 0, 0);
+  for (uint64_t u = t; u < units; u += threads) {
+    if (kStream) __stcs(dst + u, make_uint4(0, 0, 0, 0));
+    else dst[u] = make_uint4(0, 0, 0, 0);
+  }
   if (t < head) at[t] = 0;
   if (t < tail) at[bytes - 1 - t] = 0;
 }

@@ -58,7 +58,7 @@ def untouched(view, buf):
 EMBED = [  # tokens, vocab, width, pad, shift
     (1, 1, 1, 0, 0), (1, 5, 64, 0, 0), (3, 7, 100, 0, 0), (33, 100, 8, 8, 0), (65, 50, 1031, 1, 1),
     (500, 1000, 256, 64, 8), (64, 300, 4100, 4, 2), (2049, 5, 24, 0, 4), (300, 70000, 36, 0, 0),
-    (31, 9, 2, 2, 0), (4099, 31, 520, 0, 0),
+    (31, 9, 2, 2, 0), (4099, 31, 520, 0, 0), (700, 40, 333, 0, 0), (90, 60, 2050, 5, 3),
 ]
 
 
@@ -285,7 +285,8 @@ def test_expert_sort_of_few_and_odd_choices(torch_cuda, dcopy):
         assert np.array_equal(offsets.cpu().numpy(), o)
 
 
-WIDTHS = [(1, 0, 0), (8, 0, 0), (100, 4, 0), (257, 1, 1), (1024, 0, 0), (2056, 8, 8)]
+WIDTHS = [(1, 0, 0), (8, 0, 0), (17, 3, 5), (100, 4, 0), (257, 1, 1), (1024, 0, 0), (1030, 0, 0),
+          (2056, 8, 8)]
 
 
 @pytest.mark.parametrize("case", ROUTES[:10], ids=str)
