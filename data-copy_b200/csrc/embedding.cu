@@ -307,7 +307,7 @@ int dcopy_embedding_lookup(const DcopyMatrix *out, const DcopyMatrix *table,
     return with_float(out->type, [&](auto tout) {
       using TIn = typename decltype(tin)::type;
       using TOut = typename decltype(tout)::type;
-      // Shifted below 8-byte vectors (16384 rows of 1025 bf16: 25 us against 60 in single
+      // Shifted below 8-byte vectors (24390 rows of 1025 bf16: 25 us against 60 in single
       // elements; of 1025 fp32: 21 against 33).
       constexpr int kBytes = std::max(sizeof(TIn), sizeof(TOut));
       constexpr int kFull = 16 / kBytes, kLeast = 8 / kBytes;
@@ -398,7 +398,7 @@ int dcopy_embedding_grad(const DcopyMatrix *grad, const DcopyMatrix *dout, const
     return with_float(grad->type, [&](auto tout) {
       using TIn = typename decltype(tin)::type;
       using TOut = typename decltype(tout)::type;
-      // Never shifted: 16384 tokens of 1026 bf16 take 83 us in 4-byte vectors, 107 shifted.
+      // Never shifted: 24366 tokens of 1026 bf16 take 83 us in 4-byte vectors, 107 shifted.
       constexpr int kFull = 16 / std::max(sizeof(TIn), sizeof(TOut));
       const Cut cut = cut_rows(kFull, 1, grad, dout);
       p.vectors = vectors_of(grad->cols, cut);

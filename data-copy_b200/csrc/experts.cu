@@ -186,9 +186,10 @@ __global__ void __launch_bounds__(kRowThreads) combine_kernel(Route p) {
 // (1 << lx) lanes, a warp at most, take an entry: the token's row of dout meets the
 // entry's row of y.  The entries of a token are neighbours, so that its row comes from
 // L2 after the first.  (A block a token, slot after slot, with block-wide sums: 210 us
-// instead of 186 for 16384 tokens x 8 slots x 2048 bf16.)
+// instead of 187 for 16384 tokens x 8 slots x 2048 bf16.)  The bound on blocks lets the
+// compiler keep all loads of a step in flight (1501 x 2 x 1002 fp32: 9.7 us, 12.4 without).
 template <typename T, int V>
-__global__ void __launch_bounds__(kRowThreads) combine_grad_kernel(Route p) {
+__global__ void __launch_bounds__(kRowThreads, 4) combine_grad_kernel(Route p) {
   pdl_trigger_at_entry();
   pdl_wait();
   pdl_launch_dependents();
@@ -202,21 +203,23 @@ __global__ void __launch_bounds__(kRowThreads) combine_grad_kernel(Route p) {
   float dot = 0.0f;
   if (row >= 0 && (uint32_t)row < p.rows) {
     const float w = p.weights[token * p.w_pitch + slot];
-    const T *dout = static_cast<const T *>(p.dout) + token * p.dout_pitch;
-    const T *y = static_cast<const T *>(p.in) + row * p.in_pitch;
-    T *dy = static_cast<T *>(p.out) + row * p.out_pitch;
-    constexpr int U = 4;
-    for (uint32_t c0 = lane; c0 < p.vectors; c0 += U * lanes) {
+    constexpr int N = V * (int)sizeof(T), U = 4;
+    const auto *dout = reinterpret_cast<const uint8_t *>(static_cast<const T *>(p.dout) +
+                                                         token * p.dout_pitch);
+    const auto *y = reinterpret_cast<const uint8_t *>(static_cast<const T *>(p.in) +
+                                                      row * p.in_pitch);
+    auto *dy = reinterpret_cast<uint8_t *>(static_cast<T *>(p.out) + row * p.out_pitch);
+    for (uint32_t q = lane; q < p.vectors; q += U * lanes) {
       Vec<T, V> g[U], in[U];
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (c0 + u * lanes < p.vectors) {
-          in[u].load(y + (uint64_t)(c0 + u * lanes) * V);
-          g[u].load(dout + (uint64_t)(c0 + u * lanes) * V);
+        if (q + u * lanes < p.vectors) {
+          in[u].load(y + (uint64_t)(q + u * lanes) * N);
+          g[u].load(dout + (uint64_t)(q + u * lanes) * N);
         }
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (c0 + u * lanes < p.vectors) {
+        if (q + u * lanes < p.vectors) {
           float f[V];
 #pragma unroll
           for (int i = 0; i < V; ++i) {
@@ -226,7 +229,7 @@ __global__ void __launch_bounds__(kRowThreads) combine_grad_kernel(Route p) {
           }
           Vec<T, V> out;
           out.put(f);
-          out.store_cs(dy + (uint64_t)(c0 + u * lanes) * V);
+          out.store_cs(dy + (uint64_t)(q + u * lanes) * N);
         }
     }
   }
@@ -403,7 +406,7 @@ int dcopy_expert_dispatch(const DcopyMatrix *out, const DcopyMatrix *x, const in
   p.width = (uint32_t)out->cols * eb;
   const uint64_t all = (uintptr_t)out->data | (uintptr_t)x->data | p.width |
                        (out->rows > 1 ? p.out_pitch : 0) | (x->rows > 1 ? p.in_pitch : 0);
-  // Shifted below 8-byte units (16384 x 4 rows of 1025 bf16: 68 us against 145 in single
+  // Shifted below 8-byte units (24390 x 4 rows of 1025 bf16: 68 us against 145 in single
   // elements; of 1026: 66 against 101 in 4-byte units).
   const Cut cut = all % 16 == 0 ? Cut{16, false} : all % 8 == 0 ? Cut{8, false} : Cut{16, true};
   p.vectors = vectors_of(p.width, cut);
@@ -440,7 +443,7 @@ int dcopy_expert_combine(const DcopyMatrix *out, const DcopyMatrix *y, const int
   p.width = (uint32_t)out->cols;
   return with_float(out->type, [&](auto t) {
     using T = typename decltype(t)::type;
-    // Shifted where single 2-byte elements would be read (65536 choices x 1025 bf16: 104 us
+    // Shifted where single 2-byte elements would be read (97560 choices x 1025 bf16: 104 us
     // against 145); 4-byte vectors do as they are (1026: 88 us against 104 shifted).
     constexpr int kFull = 16 / sizeof(T), kLeast = 4 / sizeof(T);
     const Cut cut = cut_rows(kFull, kLeast, out, y);
@@ -500,7 +503,7 @@ int dcopy_expert_combine_grad(const DcopyMatrix *dy, const DcopyMatrix *dweights
   p.width = (uint32_t)dy->cols;
   return with_float(dy->type, [&](auto t) {
     using T = typename decltype(t)::type;
-    // Never shifted: 16384 x 4 entries of 1025 bf16 take 157 us in single elements, 182
+    // Never shifted: 24390 x 4 entries of 1025 bf16 take 138 us in single elements, 182
     // shifted.
     constexpr int kFull = 16 / sizeof(T);
     const Cut cut = cut_rows(kFull, 1, dy, dout, y);
