@@ -20,9 +20,9 @@ namespace dcopy {
 namespace {
 
 constexpr int kThreads = 256;
-// 16-byte loads a thread has in flight: 537 M bf16 elements take 487 us with 8, 521
-// with 4.
-constexpr int kUnroll = 8;
+// Bytes that a thread has in flight: 537 M bf16 elements take 487 us with 128, 521 with
+// 64.
+constexpr int kAhead = 128;
 
 // Elements of a chunk: 32 squares a thread in fp32, 0.2 % of the bytes for the table.
 constexpr uint32_t kChunk = 8192;
@@ -63,12 +63,11 @@ __device__ __forceinline__ Chunk load_chunk(const Chunk *c) {
   return u.chunk;
 }
 
-// Calls f(vector, first element) on this thread's share of a chunk: vectors of 16
-// bytes of src, U loads ahead, and single elements at the ends.  The share does not
-// depend on U.
-template <typename T, int U, typename F>
+// Calls f(vector, first element) on this thread's share of a chunk: vectors of V
+// elements, U loads ahead, and single elements at the ends.  The share does not depend
+// on U.
+template <typename T, int V, int U, typename F>
 __device__ __forceinline__ void each_vector(const Chunk &c, F &&f) {
-  constexpr uint32_t V = 16 / sizeof(T);
   const T *src = static_cast<const T *>(c.src);
   const uint32_t vectors = (c.count - c.head) / V, tail = c.head + vectors * V;
 #pragma unroll 1
@@ -106,9 +105,10 @@ __device__ __forceinline__ double block_sum(double v, double *warp_sum) {
 // (above 2^127, or so small that what underflows could count): then again in fp64.
 template <typename T>
 __device__ __forceinline__ double chunk_squares(const Chunk &c) {
+  constexpr int V = 16 / sizeof(T);
   float sum = 0.0f;
   uint32_t bits = 0;
-  each_vector<T, kUnroll>(c, [&](const auto &v, uint32_t) {
+  each_vector<T, V, kAhead / 16>(c, [&](const auto &v, uint32_t) {
 #pragma unroll
     for (int i = 0; i < v.kSize; ++i) sum = fmaf(v.get(i), v.get(i), sum);
 #pragma unroll
@@ -116,7 +116,7 @@ __device__ __forceinline__ double chunk_squares(const Chunk &c) {
   });
   if (bits == 0 || (sum >= 0x1p-90f && sum < 0x1p+127f)) return sum;
   double wide = 0.0;
-  each_vector<T, 1>(c, [&](const auto &v, uint32_t) {
+  each_vector<T, V, 1>(c, [&](const auto &v, uint32_t) {
 #pragma unroll
     for (int i = 0; i < v.kSize; ++i) wide = fma((double)v.get(i), (double)v.get(i), wide);
   });
@@ -175,12 +175,13 @@ __global__ void __launch_bounds__(kThreads) clip_kernel(List l, uint32_t parts, 
     if (k + gridDim.x < l.chunks) next = load_chunk(l.chunk + (l.chunks - 1 - k - gridDim.x));
     if (f == 1.0f && c.src == c.dst) continue;  // in place: nothing changes
     O *dst = static_cast<O *>(c.dst);
-    each_vector<T, kUnroll>(c, [&](const auto &v, uint32_t e) {
-      constexpr int V = std::decay_t<decltype(v)>::kSize;
-      float g[V];
+    constexpr int V = 16 / (sizeof(T) > sizeof(O) ? sizeof(T) : sizeof(O));
+    each_vector<T, V, kAhead / (V * sizeof(T))>(c, [&](const auto &v, uint32_t e) {
+      constexpr int kSize = std::decay_t<decltype(v)>::kSize;
+      float g[kSize];
 #pragma unroll
-      for (int i = 0; i < V; ++i) g[i] = v.get(i) * f;
-      Vec<O, V> out;
+      for (int i = 0; i < kSize; ++i) g[i] = v.get(i) * f;
+      Vec<O, kSize> out;
       out.put(g);
       out.store(dst + e);
     });

@@ -118,7 +118,7 @@ def test_embedding_grad(torch_cuda, dcopy, case, dout_type, grad_type, accumulat
 
 
 @pytest.mark.parametrize("ids", ["one", "two runs", "none", "every", "every back", "ends"])
-@pytest.mark.parametrize("n", [1, 31, 32, 33, 64, 100, 5000])
+@pytest.mark.parametrize("n", [1, 31, 32, 33, 64, 100, 511, 512, 513, 1024, 1025, 4096, 4097, 5000])
 def test_embedding_grad_runs(torch_cuda, dcopy, ids, n):
     """Runs of equal ids that begin, cross and end at every place of the sorted list."""
     vocab, width = n + 3, 40
