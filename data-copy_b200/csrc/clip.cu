@@ -233,9 +233,10 @@ List part_of(const DcopyGradList *list, uint32_t begin, uint32_t end) {
               reinterpret_cast<double *>(w), end - begin};
 }
 
-template <typename K>
-uint32_t list_grid(K kernel, uint32_t chunks) {
-  return std::min({chunks, resident_ctas(kernel, kThreads, 0), kMaxBlocks});
+// Blocks of a pass: as many as fit at once, five and four an SM.  Fixed numbers, since
+// the order of the sums hangs on them.
+uint32_t list_grid(uint32_t chunks, uint32_t per_sm) {
+  return std::min({chunks, per_sm * (uint32_t)sm_count(), kMaxBlocks});
 }
 
 // The first pass: a launch for each source type; *parts partial sums.
@@ -248,7 +249,7 @@ int run_sum(const DcopyGradList *list, uint32_t *parts, cudaStream_t s) {
     l.part += *parts;
     const int rc = with_float(kTypes[t], [&](auto tag) {
       auto k = sum_squares_kernel<typename decltype(tag)::type>;
-      const uint32_t grid = list_grid(k, l.chunks);
+      const uint32_t grid = list_grid(l.chunks, 5);
       *parts += grid;
       return launch(k, grid, dim3(kThreads), 0, s, "sum_squares_kernel", l);
     });
@@ -271,7 +272,7 @@ int run_clip(const DcopyGradList *list, uint32_t parts, const double *total, flo
     const int rc = with_float(kTypes[q / 3], [&](auto tin) {
       return with_float(kTypes[q % 3], [&](auto tout) {
         auto k = clip_kernel<typename decltype(tin)::type, typename decltype(tout)::type>;
-        return launch(k, std::max(1u, list_grid(k, l.chunks)), dim3(kThreads), 0, s, "clip_kernel",
+        return launch(k, std::max(1u, list_grid(l.chunks, 4)), dim3(kThreads), 0, s, "clip_kernel",
                       l, parts, total, max_norm, eps, norm);
       });
     });

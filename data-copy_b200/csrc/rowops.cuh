@@ -31,7 +31,7 @@ inline bool is_float(int32_t type) { return type == kF32 || type == kF16 || type
 inline bool is_index(int32_t type) { return type == kI32 || type == kI64; }
 
 // Widths beyond this are refused: the column split is the grid's y dimension.
-constexpr int64_t kMaxWidth = 1 << 24;
+constexpr int64_t kMaxWidth = 1 << 23;
 
 // Shape, pitch, type and span of one matrix argument.  `ok` tells whether the
 // type is one the operator takes.

@@ -329,7 +329,7 @@ def _expert_dispatch_fake(x, dest, source):
 def expert_combine(y: torch.Tensor, dest: torch.Tensor, source: torch.Tensor,
                    weights: Optional[torch.Tensor] = None) -> torch.Tensor:
     out = y.new_empty(dest.shape[0], y.shape[1])
-    dcopy.expert_combine(out, _dense(y), dest, None if weights is None else _dense(weights))
+    dcopy.expert_combine(out, _dense(y), dest, None if weights is None else _dense(weights.float()))
     return out
 
 
@@ -343,9 +343,10 @@ def expert_combine_backward(dout: torch.Tensor, y: torch.Tensor, dest: torch.Ten
                             source: torch.Tensor,
                             weights: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     dy = y.new_empty(y.shape)
-    dweights = weights.new_empty(weights.shape)
-    dcopy.expert_combine_grad(dy, dweights, _dense(dout), _dense(y), dest, _dense(weights), source)
-    return dy, dweights
+    dweights = weights.new_empty(weights.shape, dtype=torch.float32)  # the kernel's type
+    dcopy.expert_combine_grad(dy, dweights, _dense(dout), _dense(y), dest, _dense(weights.float()),
+                              source)
+    return dy, dweights.to(weights.dtype, copy=weights.dtype != torch.float32)
 
 
 @expert_combine_backward.register_fake

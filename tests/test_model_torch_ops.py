@@ -68,6 +68,21 @@ def test_gradients_match_autograd(ops, torch_cuda):
 
 
 @pytest.mark.gpu
+def test_weights_of_the_rows_type(ops, torch_cuda):
+    """A router in bf16: its weights count as the fp32 values they stand for, and their
+    gradient comes back in bf16."""
+    chosen, dest, source, _ = _route(ops)
+    y = torch.randn(source.numel(), 20, device="cuda").bfloat16()
+    w = torch.randn(30, 3, device="cuda").bfloat16().requires_grad_()
+    seed = torch.randn(30, 20, device="cuda").bfloat16()
+    out = ops.expert_combine(y, dest, source, w)
+    assert torch.equal(out, ops.expert_combine(y, dest, source, w.detach().float()))
+    got, = torch.autograd.grad(out, w, seed)
+    _, want = ops.expert_combine_backward(seed, y, dest, source, w.detach().float())
+    assert got.dtype == torch.bfloat16 and torch.equal(got, want.bfloat16())
+
+
+@pytest.mark.gpu
 def test_opcheck(ops, torch_cuda):
     chosen, dest, source, _ = _route(ops)
     x, w = torch.randn(30, 20, device="cuda"), torch.randn(30, 3, device="cuda")
