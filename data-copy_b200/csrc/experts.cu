@@ -20,6 +20,39 @@
 namespace dcopy {
 namespace {
 
+// The vectors of a group of tokens laid end to end over the threads of grid.y blocks, so
+// that few threads are left over whatever the width (24390 x 4 rows of 1028 bf16, 257
+// vectors: combined in 42 us, dispatched in 64; with a power of two threads a row in 64
+// and 71).  Dispatch gives narrow rows a power of two all the same: a warp that
+// writes to two rows at once is slower (260416 x 4 rows of 90 fp32: 80 us, not 58).
+struct Flat {
+  dim3 grid;
+  uint32_t group, items;  // tokens of a group, their vectors
+  FastDiv stride;         // threads of a token
+};
+
+Flat flat_tokens(uint64_t tokens, uint32_t vectors, bool whole_warps) {
+  Flat f;
+  uint32_t stride = std::max<uint32_t>(1, vectors);
+  if (whole_warps && vectors <= 64)
+    for (stride = 1; stride < vectors;) stride *= 2;
+  f.stride = FastDiv(stride);
+  // The first group from one block's worth on that leaves less than 5 % over.
+  const uint32_t least = std::max<uint32_t>(1, kRowThreads / stride);
+  double best = 0.0;
+  f.group = 1;
+  for (uint32_t g = least; g < least + 16 && best < 0.95; ++g) {
+    const uint64_t items = (uint64_t)g * stride;
+    const uint64_t blocks = (items + kRowThreads - 1) / kRowThreads;
+    const double used = (double)items / (double)(blocks * kRowThreads);
+    if (used > best + 0.01) best = used, f.group = g;
+  }
+  f.items = f.group * stride;
+  f.grid = dim3((unsigned)((tokens + f.group - 1) / f.group),
+                (f.items + kRowThreads - 1) / kRowThreads);
+  return f;
+}
+
 struct Route {
   void *out;              // dispatch: rows in expert order; combine: tokens
   const void *in;         // dispatch: tokens; combine: rows in expert order
@@ -28,36 +61,52 @@ struct Route {
   int64_t out_pitch, in_pitch, dout_pitch, w_pitch, dw_pitch;
   const int32_t *dest, *source;
   const float *weights;
-  uint32_t tokens, slots, rows, width, vectors, unused_blocks;
+  uint32_t tokens, slots, rows, width, vectors, unused_blocks, unused_rows;
+  Flat flat;
   FastDiv by_slots;
   int lx;
 };
 
-// Rows of the buffer in expert order that hold no entry are zeroed by the first
-// blocks of the grid, kUnusedRows rows each, a warp kWarpRows of them: padding comes in
-// runs of rows, and ahead of the others these blocks do not trail the kernel.  More rows
-// a warp take longer over a run (655 x 4 entries, experts padded to 128: 6.5 us with 8,
-// 15 with 32), fewer cost blocks that find nothing (65536 x 4 x 2048: 3 % with 4).
-constexpr uint32_t kWarpRows = 8, kUnusedRows = kWarpRows * (kRowThreads / 32);
+// Rows of the buffer in expert order that hold no entry are zeroed by the first blocks
+// of the grid, a warp unused_rows of them: padding comes in runs of rows, and ahead of
+// the others these blocks do not trail the kernel.  More rows a warp take longer over a
+// run (655 x 4 entries, experts padded to 128: 4.3 us with 8, 7.1 with 32), fewer cost
+// blocks that find nothing (262144 x 2 x 1024: 246 us with 8, 239 with 32), so the rows
+// a warp grow with the buffer.
+uint32_t unused_rows_of(uint64_t rows) {
+  uint32_t n = 8;
+  while (n < 32 && rows > 1024ull * n * (kRowThreads / 32)) n *= 2;
+  return n;
+}
 
 __device__ __forceinline__ void zero_unused(const Route &p, uint32_t elem_bytes) {
   const uint32_t lane = threadIdx.x % 32;
-  const uint32_t r0 = blockIdx.x * kUnusedRows + threadIdx.x / 32 * kWarpRows;
-  const bool mine = lane < kWarpRows && r0 + lane < p.rows && lane % gridDim.y == blockIdx.y;
+  const uint32_t r0 = (blockIdx.x * (kRowThreads / 32) + threadIdx.x / 32) * p.unused_rows;
+  const bool mine = lane < p.unused_rows && r0 + lane < p.rows && lane % gridDim.y == blockIdx.y;
   uint32_t empty = __ballot_sync(~0u, mine && p.source[r0 + lane] < 0);
+  if (!empty) return;
+  const uint64_t pitch = p.out_pitch * elem_bytes;
+  const uint32_t bytes = p.width * elem_bytes, units = bytes / 16;
+  uint8_t *rows = static_cast<uint8_t *>(p.out) + r0 * pitch;
+  const bool granules = (reinterpret_cast<uintptr_t>(rows) | pitch | bytes) % 16 == 0;
   for (; empty; empty &= empty - 1) {
-    const uint64_t row = r0 + __ffs(empty) - 1;
-    zero_bytes<true>(static_cast<uint8_t *>(p.out) + row * p.out_pitch * elem_bytes,
-                     (uint64_t)p.width * elem_bytes, lane, 32);
+    uint8_t *row = rows + (__ffs(empty) - 1) * pitch;
+    if (granules) {
+      for (uint32_t u = lane; u < units; u += 32)
+        __stcs(reinterpret_cast<uint4 *>(row) + u, make_uint4(0, 0, 0, 0));
+    } else {
+      zero_bytes<true>(row, bytes, lane, 32);
+    }
   }
 }
 
-// The thread's token (or p.tokens and more) and its first vector.
-__device__ __forceinline__ uint32_t my_token(const Route &p) {
-  return (blockIdx.x - p.unused_blocks) * (kRowThreads >> p.lx) + (threadIdx.x >> p.lx);
-}
-__device__ __forceinline__ uint32_t my_vector(const Route &p) {
-  return (blockIdx.y << p.lx) + (threadIdx.x & ((1u << p.lx) - 1));
+// The thread's token and vector; false when it has none.
+__device__ __forceinline__ bool my_vector(const Route &p, uint32_t *token, uint32_t *q) {
+  const uint32_t i = blockIdx.y * kRowThreads + threadIdx.x;
+  const uint32_t r = p.flat.stride.div(i);
+  *token = (blockIdx.x - p.unused_blocks) * p.flat.group + r;
+  *q = i - r * p.flat.stride.d;
+  return i < p.flat.items && *token < p.tokens && *q < p.vectors;
 }
 
 // Rows moved as bytes (widths and pitches in bytes): units of N bytes, read once for
@@ -68,8 +117,8 @@ __global__ void __launch_bounds__(kRowThreads) dispatch_kernel(Route p) {
   pdl_wait();
   pdl_launch_dependents();
   if (blockIdx.x < p.unused_blocks) return zero_unused(p, 1);
-  const uint32_t token = my_token(p), q = my_vector(p);
-  if (token >= p.tokens || q >= p.vectors) return;
+  uint32_t token, q;
+  if (!my_vector(p, &token, &q)) return;
   Words<N> in;
   in.load(static_cast<const uint8_t *>(p.in) + token * p.in_pitch + (uint64_t)q * N);
   const int32_t *dest = p.dest + (uint64_t)token * p.slots;
@@ -87,8 +136,8 @@ __global__ void __launch_bounds__(kRowThreads) dispatch_shift_kernel(Route p) {
   pdl_wait();
   pdl_launch_dependents();
   if (blockIdx.x < p.unused_blocks) return zero_unused(p, 1);
-  const uint32_t token = my_token(p), q = my_vector(p);
-  if (token >= p.tokens || q >= p.vectors) return;
+  uint32_t token, q;
+  if (!my_vector(p, &token, &q)) return;
   const uint8_t *src = static_cast<const uint8_t *>(p.in) + token * p.in_pitch;
   const int32_t *dest = p.dest + (uint64_t)token * p.slots;
   for (uint32_t j = 0; j < p.slots; ++j) {
@@ -114,8 +163,8 @@ __global__ void __launch_bounds__(kRowThreads) dispatch_weighted_kernel(Route p)
   pdl_wait();
   pdl_launch_dependents();
   if (blockIdx.x < p.unused_blocks) return zero_unused(p, sizeof(T));
-  const uint32_t token = my_token(p), q = my_vector(p);
-  if (token >= p.tokens || q >= p.vectors) return;
+  uint32_t token, q;
+  if (!my_vector(p, &token, &q)) return;
   const T *src = static_cast<const T *>(p.in) + token * p.in_pitch;
   Vec<T, V> in;
   if (!kShift) load_columns<T, V, kShift>(in, src, (int32_t)(q * V), p.width);
@@ -141,8 +190,8 @@ __global__ void __launch_bounds__(kRowThreads) combine_kernel(Route p) {
   pdl_trigger_at_entry();
   pdl_wait();
   pdl_launch_dependents();
-  const uint32_t token = my_token(p), q = my_vector(p);
-  if (token >= p.tokens || q >= p.vectors) return;
+  uint32_t token, q;
+  if (!my_vector(p, &token, &q)) return;
   T *dst = static_cast<T *>(p.out) + token * p.out_pitch;
   const int32_t c = (int32_t)(q * V) - row_lead<T, V, kShift>(dst);
   if (c >= (int32_t)p.width) return;
@@ -188,7 +237,8 @@ __global__ void __launch_bounds__(kRowThreads, 4) combine_grad_kernel(Route p) {
   pdl_launch_dependents();
   if (blockIdx.x < p.unused_blocks)
     return zero_unused(p, sizeof(T));
-  const uint32_t entry = my_token(p);
+  const uint32_t entry =
+      (blockIdx.x - p.unused_blocks) * (kRowThreads >> p.lx) + (threadIdx.x >> p.lx);
   const uint32_t lanes = 1u << p.lx, lane = threadIdx.x & (lanes - 1);
   const uint32_t token = p.by_slots.div(entry), slot = entry - token * p.slots;
   const bool there = token < p.tokens;
@@ -262,19 +312,18 @@ int check_width(const DcopyMatrix *a, const DcopyMatrix *b, const char *what) {
   return DCOPY_OK;
 }
 
-uint32_t unused_blocks(const int32_t *source, uint64_t rows);
-
-// The grid of the kernels whose threads take a vector of a token's row.
-dim3 token_grid(Route &p, const int32_t *source) {
-  RowSplit split = split_rows(p.tokens, p.vectors, 1);
-  p.lx = split.lx;
-  p.unused_blocks = unused_blocks(source, p.rows);
-  split.grid.x += p.unused_blocks;
-  return split.grid;
+// Blocks ahead of the others that zero the rows without an entry.
+void plan_unused(Route &p, const int32_t *source) {
+  p.unused_rows = unused_rows_of(p.rows);
+  const uint32_t block = p.unused_rows * (kRowThreads / 32);
+  p.unused_blocks = source ? (p.rows + block - 1) / block : 0;
 }
 
-uint32_t unused_blocks(const int32_t *source, uint64_t rows) {
-  return source ? (uint32_t)((rows + kUnusedRows - 1) / kUnusedRows) : 0;
+// The grid of the kernels whose threads take a vector of a token's row.
+dim3 token_grid(Route &p, const int32_t *source, bool whole_warps) {
+  p.flat = flat_tokens(p.tokens, p.vectors, whole_warps);
+  plan_unused(p, source);
+  return dim3(p.flat.grid.x + p.unused_blocks, std::max(1u, p.flat.grid.y));
 }
 
 }  // namespace
@@ -385,7 +434,7 @@ int dcopy_expert_dispatch(const DcopyMatrix *out, const DcopyMatrix *x, const in
       constexpr int kFull = 16 / sizeof(T), kLeast = 8 / sizeof(T);
       const Cut cut = cut_rows(kFull, kLeast, out, x);
       p.vectors = vectors_of(out->cols, cut);
-      const dim3 grid = token_grid(p, source);
+      const dim3 grid = token_grid(p, source, true);
       if (grid.x == 0) return (int)DCOPY_OK;
       return with_cut<kFull, kLeast>(cut, [&](auto v, auto shift) {
         return launch_grid(dispatch_weighted_kernel<T, v(), shift()>, grid, dim3(kRowThreads), 0,
@@ -403,7 +452,7 @@ int dcopy_expert_dispatch(const DcopyMatrix *out, const DcopyMatrix *x, const in
   // elements; of 1026: 66 against 101 in 4-byte units).
   const Cut cut = all % 16 == 0 ? Cut{16, false} : all % 8 == 0 ? Cut{8, false} : Cut{16, true};
   p.vectors = vectors_of(p.width, cut);
-  const dim3 grid = token_grid(p, source);
+  const dim3 grid = token_grid(p, source, true);
   if (grid.x == 0) return DCOPY_OK;
   auto k = cut.shift ? dispatch_shift_kernel : cut.v == 16 ? dispatch_kernel<16> : dispatch_kernel<8>;
   return launch_grid(k, grid, dim3(kRowThreads), 0, stream, "dispatch_kernel", p);
@@ -441,7 +490,7 @@ int dcopy_expert_combine(const DcopyMatrix *out, const DcopyMatrix *y, const int
     constexpr int kFull = 16 / sizeof(T), kLeast = 4 / sizeof(T);
     const Cut cut = cut_rows(kFull, kLeast, out, y);
     p.vectors = vectors_of(out->cols, cut);
-    const dim3 grid = token_grid(p, nullptr);
+    const dim3 grid = token_grid(p, nullptr, false);
     return with_cut<kFull, kLeast>(cut, [&](auto v, auto shift) {
       return launch_grid(combine_kernel<T, v(), shift()>, grid, dim3(kRowThreads), 0, stream,
                          "combine_kernel", p);
@@ -489,7 +538,7 @@ int dcopy_expert_combine_grad(const DcopyMatrix *dy, const DcopyMatrix *dweights
   p.tokens = (uint32_t)dout->rows;
   p.slots = (uint32_t)slots;
   p.rows = (uint32_t)dy->rows;
-  p.unused_blocks = unused_blocks(source, dy->rows);
+  plan_unused(p, source);
   p.by_slots = FastDiv((uint32_t)std::max<int64_t>(1, slots));
   const uint64_t entries = (uint64_t)p.tokens * p.slots;
   p.width = (uint32_t)dy->cols;
