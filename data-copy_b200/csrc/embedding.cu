@@ -18,13 +18,6 @@
 namespace dcopy {
 namespace {
 
-__device__ __forceinline__ int64_t read_id(const KeySource &k, uint32_t e) {
-  const uint32_t r = k.cols.div(e);
-  const int64_t at = (int64_t)r * k.pitch + (e - r * k.cols.d);
-  return (k.wide ? static_cast<const int64_t *>(k.ids)[at]
-                 : (int64_t)static_cast<const int32_t *>(k.ids)[at]) - k.first;
-}
-
 struct Lookup {
   void *out;
   const void *table;

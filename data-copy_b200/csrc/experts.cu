@@ -22,7 +22,7 @@ namespace {
 
 // The vectors of a group of tokens laid end to end over the threads of grid.y blocks, so
 // that few threads are left over whatever the width (24390 x 4 rows of 1028 bf16, 257
-// vectors: combined in 42 us, dispatched in 64; with a power of two threads a row in 64
+// vectors: combined in 42 us, dispatched in 54; with a power of two threads a row in 64
 // and 71).  Dispatch gives narrow rows a power of two all the same: a warp that
 // writes to two rows at once is slower (260416 x 4 rows of 90 fp32: 80 us, not 58).
 struct Flat {
@@ -448,8 +448,9 @@ int dcopy_expert_dispatch(const DcopyMatrix *out, const DcopyMatrix *x, const in
   p.width = (uint32_t)out->cols * eb;
   const uint64_t all = (uintptr_t)out->data | (uintptr_t)x->data | p.width |
                        (out->rows > 1 ? p.out_pitch : 0) | (x->rows > 1 ? p.in_pitch : 0);
-  // Shifted below 8-byte units (24390 x 4 rows of 1025 bf16: 68 us against 145 in single
-  // elements; of 1026: 66 against 101 in 4-byte units).
+  // Shifted below 8-byte units (24390 x 4 rows of 1025 bf16: 60 us against 145 in single
+  // elements; of 1026: 58 against 101 in 4-byte units; of 1028 in 8-byte units 54 against 56
+  // shifted).
   const Cut cut = all % 16 == 0 ? Cut{16, false} : all % 8 == 0 ? Cut{8, false} : Cut{16, true};
   p.vectors = vectors_of(p.width, cut);
   const dim3 grid = token_grid(p, source, true);
@@ -485,8 +486,8 @@ int dcopy_expert_combine(const DcopyMatrix *out, const DcopyMatrix *y, const int
   p.width = (uint32_t)out->cols;
   return with_float(out->type, [&](auto t) {
     using T = typename decltype(t)::type;
-    // Shifted where single 2-byte elements would be read (97560 choices x 1025 bf16: 104 us
-    // against 145); 4-byte vectors do as they are (1026: 88 us against 104 shifted).
+    // Shifted where single 2-byte elements would be read (24390 x 4 choices of 1025 bf16: 84
+    // us against 132); 4-byte vectors do as they are (1026: 70 us against 86 shifted).
     constexpr int kFull = 16 / sizeof(T), kLeast = 4 / sizeof(T);
     const Cut cut = cut_rows(kFull, kLeast, out, y);
     p.vectors = vectors_of(out->cols, cut);

@@ -28,11 +28,7 @@ constexpr uint32_t kMaxBins = 1 << kExpertBits;
 constexpr uint32_t kOneTile = 8 * kThreads;
 
 __device__ __forceinline__ uint32_t entry_key(const KeySource &k, uint32_t e) {
-  const uint32_t r = k.cols.div(e);
-  const int64_t at = (int64_t)r * k.pitch + (e - r * k.cols.d);
-  const int64_t id = (k.wide ? static_cast<const int64_t *>(k.ids)[at]
-                             : (int64_t)static_cast<const int32_t *>(k.ids)[at]) -
-                     k.first;
+  const int64_t id = read_id(k, e);
   return id >= 0 && id < (int64_t)k.keys ? (uint32_t)id : k.keys;
 }
 

@@ -21,6 +21,15 @@ struct KeySource {
   FastDiv cols;
 };
 
+// The e-th id less `first`.
+__device__ __forceinline__ int64_t read_id(const KeySource &k, uint32_t e) {
+  const uint32_t r = k.cols.div(e);
+  const int64_t at = (int64_t)r * k.pitch + (e - r * k.cols.d);
+  return (k.wide ? static_cast<const int64_t *>(k.ids)[at]
+                 : (int64_t)static_cast<const int32_t *>(k.ids)[at]) -
+         k.first;
+}
+
 // Rows [begin, end) to zero beside the sort: its few blocks leave most SMs idle, so
 // each of its launches also clears some, the last ones first.  (Vocabularies have their
 // frequent ids in front, and rows that tokens have are written again.)
