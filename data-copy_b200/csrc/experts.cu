@@ -110,7 +110,10 @@ __device__ __forceinline__ bool my_vector(const Route &p, uint32_t *token, uint3
 }
 
 // Rows moved as bytes (widths and pitches in bytes): units of N bytes, read once for
-// all slots.
+// all slots.  Bound by HBM, almost all of it writes: 16384 tokens x 8 slots of 8 KB go
+// out at 6.3 TB/s (192 us), 147328 rows with the padding of 128 experts to 128 rows at
+// 6.2 TB/s.  Fetching each row of the buffer from its token instead, so that rows are
+// written front to back, reads every token's row 8 times from L2 and took 204 us.
 template <int N>
 __global__ void __launch_bounds__(kRowThreads) dispatch_kernel(Route p) {
   pdl_trigger_at_entry();
@@ -185,6 +188,9 @@ __global__ void __launch_bounds__(kRowThreads) dispatch_weighted_kernel(Route p)
   }
 }
 
+// A thread sums one vector of a token over its slots, four rows in flight, and writes it
+// once.  Bound by HBM: 8191 x 4 x 5120 fp16 (a tenth dropped, 386 MB) take 63 us, 6.1
+// TB/s.  Registers decide: at 64 a thread (four blocks an SM) it took 72 us.
 template <typename T, int V, bool kShift>
 __global__ void __launch_bounds__(kRowThreads) combine_kernel(Route p) {
   pdl_trigger_at_entry();
@@ -227,7 +233,8 @@ __global__ void __launch_bounds__(kRowThreads) combine_kernel(Route p) {
 
 // (1 << lx) lanes, a warp at most, take an entry: the token's row of dout meets the
 // entry's row of y.  The entries of a token are neighbours, so that its row comes from
-// L2 after the first.  (A block a token, slot after slot, with block-wide sums: 210 us
+// L2 after the first.  Bound by HBM: 16384 x 8 x 2048 bf16 (1.14 GB) take 187 us, 6.1
+// TB/s.  (A block a token, slot after slot, with block-wide sums: 210 us
 // instead of 187 for 16384 tokens x 8 slots x 2048 bf16.)  The bound on blocks lets the
 // compiler keep all loads of a step in flight (1501 x 2 x 1002 fp32: 9.7 us, 12.4 without).
 template <typename T, int V>

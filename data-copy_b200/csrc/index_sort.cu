@@ -8,6 +8,10 @@
 // so the result is the same every time.  Experts fit one digit of up to 10 bits; token
 // ids take two of up to 9 bits below 2^18 and three below 2^27.  What fits one tile
 // takes one launch for all digits.
+//
+// Bound by latency, not bytes: a launch of a pass takes 4 to 5 us (counts) and 10 us
+// (places) for 131072 choices, 2.1 MB.  Most of the placing is adding up the tiles'
+// counts, 8 loads ahead (one digit a warp and four ahead: 23 us for 512 digits).
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -315,7 +319,7 @@ __global__ void __launch_bounds__(kThreads) one_tile_kernel(Pass p) {
 }
 
 // Entries a thread ranks.  Few keep many tiles (SMs) at work, many keep the tiles'
-// counts, which every tile reads, below the entries: 131072 entries are sorted in 10 us
+// counts, which every tile reads, below the entries: 131072 choices are placed in 10 us
 // with 2 and 15 us with 8.
 int items_of(uint64_t n) { return n <= 128 * 2 * kThreads ? 2 : n <= 1024 * 8 * kThreads ? 8 : 32; }
 uint32_t tiles_of(uint64_t n) {
