@@ -99,11 +99,10 @@ __device__ __forceinline__ void zero_but(const Fill &f, uint64_t row0, uint64_t 
   for (uint32_t w = 0; w < kRowThreads / 32; ++w) any |= touched[w];
   if (!any && f.pitch == f.bytes)
     return zero_bytes(f.dst + row0 * f.pitch, (row1 - row0) * f.bytes, threadIdx.x, kRowThreads);
-  for (uint64_t r = row0 + threadIdx.x / 32; r < row1; r += kRowThreads / 32) {
-    const uint32_t k = (uint32_t)(r - row0);
+  const uint32_t unit = zero_unit(f.dst, f.pitch, f.bytes);
+  for (uint32_t k = threadIdx.x / 32; k < (uint32_t)(row1 - row0); k += kRowThreads / 32)
     if (!(touched[k / 32] >> k % 32 & 1))
-      zero_bytes(f.dst + r * f.pitch, f.bytes, threadIdx.x % 32, 32);
-  }
+      zero_row(f.dst + (row0 + k) * f.pitch, (uint32_t)f.bytes, unit, threadIdx.x % 32);
 }
 
 __device__ __forceinline__ void touch(uint32_t *touched, uint32_t row) {
@@ -227,7 +226,7 @@ __global__ void __launch_bounds__(kRowThreads) few_sum_kernel(Grad p, KeySource 
 // began earlier) or tail (it begins here and goes on).  Rows of kAhead tokens are
 // fetched before the first is added.  Sums in fp32, one rounding when a row is written.
 // With the zeroing that goes along, bound by HBM: 16384 tokens, 131072 x 4096 bf16 move
-// 0.94 GB in 141 us (6.6 TB/s) here and the whole gradient takes 193 us.
+// 0.94 GB in 141 us (6.6 TB/s) here and the whole gradient takes 190 us.
 template <typename TIn, typename TOut, int V, bool kAdd>
 __global__ void __launch_bounds__(kRowThreads) piece_sum_kernel(Grad p) {
   // The ids of the block's pieces, one before and one behind; positions.
@@ -291,7 +290,7 @@ __global__ void __launch_bounds__(kRowThreads) piece_sum_kernel(Grad p) {
 // Bound by the latency of the longest run (an id that 6 % of 16384 tokens have: 17 us),
 // which the zeroing beside it hides.
 template <typename TOut, int V, bool kAdd>
-__global__ void __launch_bounds__(kRowThreads) piece_join_kernel(Grad p) {
+__global__ void __launch_bounds__(kRowThreads, 4) piece_join_kernel(Grad p) {
   pdl_trigger_at_entry();
   pdl_wait();
   pdl_launch_dependents();
@@ -310,7 +309,9 @@ __global__ void __launch_bounds__(kRowThreads) piece_join_kernel(Grad p) {
   part.load(p.tail + (uint64_t)piece * p.width + at);
 #pragma unroll
   for (int v = 0; v < V; ++v) sum[v] = part.get(v);
-  constexpr int kAhead = 8;  // 16: 40 us instead of 26 for 56403 tokens x 256
+  // 32 floats a thread at most: with 64, two blocks fit an SM and the zeroing beside the
+  // sums is slower for it (194 us instead of 190 for the gradient above).
+  constexpr int kAhead = V == 8 ? 4 : 8;
   bool on = true;
   for (uint32_t q = piece + 1; on && q < p.pieces; q += kAhead) {
     Vec<float, V> head[kAhead];

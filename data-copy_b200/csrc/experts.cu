@@ -86,18 +86,10 @@ __device__ __forceinline__ void zero_unused(const Route &p, uint32_t elem_bytes)
   uint32_t empty = __ballot_sync(~0u, mine && p.source[r0 + lane] < 0);
   if (!empty) return;
   const uint64_t pitch = p.out_pitch * elem_bytes;
-  const uint32_t bytes = p.width * elem_bytes, units = bytes / 16;
+  const uint32_t bytes = p.width * elem_bytes, unit = zero_unit(p.out, pitch, bytes);
   uint8_t *rows = static_cast<uint8_t *>(p.out) + r0 * pitch;
-  const bool granules = (reinterpret_cast<uintptr_t>(rows) | pitch | bytes) % 16 == 0;
-  for (; empty; empty &= empty - 1) {
-    uint8_t *row = rows + (__ffs(empty) - 1) * pitch;
-    if (granules) {
-      for (uint32_t u = lane; u < units; u += 32)
-        __stcs(reinterpret_cast<uint4 *>(row) + u, make_uint4(0, 0, 0, 0));
-    } else {
-      zero_bytes<true>(row, bytes, lane, 32);
-    }
-  }
+  for (; empty; empty &= empty - 1)
+    zero_row<true>(rows + (__ffs(empty) - 1) * pitch, bytes, unit, lane);
 }
 
 // The thread's token and vector; false when it has none.

@@ -188,6 +188,8 @@ __global__ void __launch_bounds__(kThreads) tile_place_kernel(Pass p, ExpertOut 
   pdl_wait();
   pdl_launch_dependents();
   const uint32_t e0 = (blockIdx.x * kThreads + warp * 32) * kItems + lane;
+  if (kExperts && p.tiles == 1)  // padding: what is not written below, behind a barrier
+    for (uint32_t r = threadIdx.x; r < o.rows; r += kThreads) o.source[r] = -1;
   uint32_t key[kItems], digit[kItems], rank[kItems];
 #pragma unroll
   for (int i = 0; i < kItems; ++i) {
@@ -240,12 +242,12 @@ __global__ void __launch_bounds__(kThreads) tile_place_kernel(Pass p, ExpertOut 
       base[d] = at + earlier;
       if (kExperts) {
         if (blockIdx.x == 0) o.offsets[d] = (int32_t)at;  // the last one: all rows in use
-        if (d + 1 < p.bins)
+        if (d + 1 < p.bins && p.tiles > 1)
           for (uint32_t r = at + mine + blockIdx.x; r < at + room; r += p.tiles) o.source[r] = -1;
       }
     }
   }
-  if (kExperts)
+  if (kExperts && p.tiles > 1)
     for (uint32_t r = carry + blockIdx.x * kThreads + threadIdx.x; r < o.rows;
          r += p.tiles * kThreads)
       o.source[r] = -1;

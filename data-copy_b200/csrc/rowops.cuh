@@ -362,6 +362,34 @@ __device__ __forceinline__ void zero_bytes(uint8_t *at, uint64_t bytes, uint32_t
   if (t < tail) at[bytes - 1 - t] = 0;
 }
 
+// For rows that a warp zeroes one after the other.  Rows of up to 512 bytes are many, so
+// that instructions count: units of 16 to 1 bytes that all rows start on, no ends.  Wider
+// rows go by zero_bytes (0) unless they are whole granules.
+__device__ __forceinline__ uint32_t zero_unit(const void *base, uint64_t pitch, uint64_t bytes) {
+  const uint32_t all = (uint32_t)(reinterpret_cast<uintptr_t>(base) | pitch | bytes);
+  const uint32_t unit = all % 16 == 0 ? 16 : all & -all;
+  return unit == 16 || bytes <= 512 ? unit : 0;
+}
+template <bool kStream = false>
+__device__ __forceinline__ void zero_row(uint8_t *row, uint32_t bytes, uint32_t unit,
+                                         uint32_t lane) {
+  if (unit == 0) return zero_bytes<kStream>(row, bytes, lane, 32);
+  for (uint32_t at = lane * unit; at < bytes; at += 32 * unit) {
+    if (unit == 16) {
+      if (kStream) __stcs(reinterpret_cast<uint4 *>(row + at), make_uint4(0, 0, 0, 0));
+      else *reinterpret_cast<uint4 *>(row + at) = make_uint4(0, 0, 0, 0);
+    } else if (unit == 8) {
+      *reinterpret_cast<uint2 *>(row + at) = make_uint2(0, 0);
+    } else if (unit == 4) {
+      *reinterpret_cast<uint32_t *>(row + at) = 0;
+    } else if (unit == 2) {
+      *reinterpret_cast<uint16_t *>(row + at) = 0;
+    } else {
+      row[at] = 0;
+    }
+  }
+}
+
 template <typename T>
 struct TypeTag {
   using type = T;
