@@ -138,11 +138,11 @@ __device__ __forceinline__ void zero_untouched(const Grad &p, uint32_t block) {
   zero_but(p.fill, row0, row1, touched);
 }
 
+// round(scale * sum), added to what the row held (`old`) with kAdd.
 template <typename T, int V, bool kAdd>
-__device__ __forceinline__ void write_row(T *row, uint32_t c, const float (&sum)[V], float scale) {
+__device__ __forceinline__ void write_row(T *row, uint32_t c, const float (&sum)[V], float scale,
+                                          const Vec<T, V> &old) {
   float f[V];
-  Vec<T, V> old;
-  if constexpr (kAdd) old.load_plain(row + (uint64_t)c * V);
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     f[i] = sum[i] * scale;
@@ -151,6 +151,11 @@ __device__ __forceinline__ void write_row(T *row, uint32_t c, const float (&sum)
   Vec<T, V> out;
   out.put(f);
   out.store(row + (uint64_t)c * V);
+}
+
+template <typename T, int V, bool kAdd>
+__device__ __forceinline__ void load_old(Vec<T, V> &old, const T *row, uint32_t c) {
+  if constexpr (kAdd) old.load_plain(row + (uint64_t)c * V);
 }
 
 // At most kFew tokens: no sort.  A block takes a token and some columns; where the token
@@ -218,7 +223,10 @@ __global__ void __launch_bounds__(kRowThreads) few_sum_kernel(Grad p, KeySource 
         for (int v = 0; v < V; ++v) sum[v] += in[j].get(v);
       }
   }
-  write_row<TOut, V, kAdd>(static_cast<TOut *>(p.grad) + key * p.grad_pitch, c, sum, p.scale);
+  TOut *row = static_cast<TOut *>(p.grad) + key * p.grad_pitch;
+  Vec<TOut, V> old;
+  load_old<TOut, V, kAdd>(old, row, c);
+  write_row<TOut, V, kAdd>(row, c, sum, p.scale, old);
 }
 
 // One piece of the sorted list: runs of equal ids that lie inside it are summed and
@@ -257,10 +265,18 @@ __global__ void __launch_bounds__(kRowThreads) piece_sum_kernel(Grad p) {
   constexpr int kAhead = 8;
   for (uint32_t i0 = 0; i0 < count && key < p.keys; i0 += kAhead) {
     Vec<TIn, V> in[kAhead];
+    // What is added to, fetched for the rows whose run ends here (2047 tokens, 32000 x
+    // 4096: 21 us instead of 25, as no run waits for its own load).
+    Vec<TOut, V> old[kAhead];
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j)
-      if (i0 + j < count && keys[local + i0 + j + 1] < p.keys)
+    for (int j = 0; j < kAhead; ++j) {
+      const uint32_t id = keys[local + i0 + j + 1];
+      if (i0 + j < count && id < p.keys) {
         in[j].load(dout + (int64_t)places[local + i0 + j] * p.dout_pitch);
+        if (keys[local + i0 + j + 2] != id)
+          load_old<TOut, V, kAdd>(old[j], grad + id * p.grad_pitch, c);
+      }
+    }
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
       if (i0 + j >= count || key >= p.keys) break;
@@ -274,7 +290,7 @@ __global__ void __launch_bounds__(kRowThreads) piece_sum_kernel(Grad p) {
           out.put(sum);
           out.store(part + (uint64_t)piece * p.width + (uint64_t)c * V);
         } else {
-          write_row<TOut, V, kAdd>(grad + key * p.grad_pitch, c, sum, p.scale);
+          write_row<TOut, V, kAdd>(grad + key * p.grad_pitch, c, sum, p.scale, old[j]);
         }
 #pragma unroll
         for (int v = 0; v < V; ++v) sum[v] = 0.0f;
@@ -330,7 +346,10 @@ __global__ void __launch_bounds__(kRowThreads, 4) piece_join_kernel(Grad p) {
       }
     }
   }
-  write_row<TOut, V, kAdd>(static_cast<TOut *>(p.grad) + key * p.grad_pitch, c, sum, p.scale);
+  TOut *row = static_cast<TOut *>(p.grad) + key * p.grad_pitch;
+  Vec<TOut, V> old;
+  load_old<TOut, V, kAdd>(old, row, c);
+  write_row<TOut, V, kAdd>(row, c, sum, p.scale, old);
 }
 
 int id_source(const DcopyMatrix *ids, int64_t first, int64_t keys, KeySource *src) {
