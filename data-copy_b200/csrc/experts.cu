@@ -72,8 +72,12 @@ struct Route {
 // the others these blocks do not trail the kernel.  More rows a warp take longer over a
 // run (655 x 4 entries, experts padded to 128: 4.3 us with 8, 7.1 with 32), fewer cost
 // blocks that find nothing (262144 x 2 x 1024: 246 us with 8, 239 with 32), so the rows
-// a warp grow with the buffer.
-uint32_t unused_rows_of(uint64_t rows) {
+// a warp grow with the buffer.  Where an eighth of the rows or more must be empty, a warp
+// takes 16 KB of them at most (10176 rows of 20 KB, 2556 in use: 46 us, with 8 rows a
+// warp 55).
+uint32_t unused_rows_of(uint64_t rows, uint64_t entries, uint64_t row_bytes) {
+  if (rows > entries + rows / 8)
+    return (uint32_t)std::clamp<uint64_t>((16 << 10) / std::max<uint64_t>(1, row_bytes), 1, 8);
   uint32_t n = 8;
   while (n < 32 && rows > 1024ull * n * (kRowThreads / 32)) n *= 2;
   return n;
@@ -86,7 +90,8 @@ __device__ __forceinline__ void zero_unused(const Route &p, uint32_t elem_bytes)
   uint32_t empty = __ballot_sync(~0u, mine && p.source[r0 + lane] < 0);
   if (!empty) return;
   const uint64_t pitch = p.out_pitch * elem_bytes;
-  const uint32_t bytes = p.width * elem_bytes, unit = zero_unit(p.out, pitch, bytes);
+  const uint32_t bytes = p.width * elem_bytes;
+  const uint32_t unit = zero_unit(p.out, pitch, bytes);
   uint8_t *rows = static_cast<uint8_t *>(p.out) + r0 * pitch;
   for (; empty; empty &= empty - 1)
     zero_row<true>(rows + (__ffs(empty) - 1) * pitch, bytes, unit, lane);
@@ -223,8 +228,8 @@ __global__ void __launch_bounds__(kRowThreads) combine_kernel(Route p) {
   store_columns<T, V, kShift>(out, dst, c, p.width);
 }
 
-// (1 << lx) lanes, a warp at most, take an entry: the token's row of dout meets the
-// entry's row of y.  The entries of a token are neighbours, so that its row comes from
+// (1 << lx) lanes take an entry, a warp at most or, where entries are few, a block: the
+// token's row of dout meets the entry's row of y.  The entries of a token are neighbours, so that its row comes from
 // L2 after the first.  Bound by HBM: 16384 x 8 x 2048 bf16 (1.14 GB) take 187 us, 6.1
 // TB/s.  (A block a token, slot after slot, with block-wide sums: 210 us
 // instead of 187 for 16384 tokens x 8 slots x 2048 bf16.)  The bound on blocks lets the
@@ -275,7 +280,14 @@ __global__ void __launch_bounds__(kRowThreads, 4) combine_grad_kernel(Route p) {
         }
     }
   }
-  for (uint32_t o = lanes / 2; o; o /= 2) dot += __shfl_xor_sync(~0u, dot, o);
+  for (uint32_t o = min(lanes, 32u) / 2; o; o /= 2) dot += __shfl_xor_sync(~0u, dot, o);
+  if (lanes > 32) {  // the whole block's
+    __shared__ float part[kRowThreads / 32];
+    if (lane % 32 == 0) part[lane / 32] = dot;
+    __syncthreads();
+    dot = 0.0f;
+    for (uint32_t w = 0; w < kRowThreads / 32; ++w) dot += part[w];
+  }
   if (lane == 0 && there) p.dweights[token * p.dw_pitch + slot] = dot;
 }
 
@@ -312,16 +324,16 @@ int check_width(const DcopyMatrix *a, const DcopyMatrix *b, const char *what) {
 }
 
 // Blocks ahead of the others that zero the rows without an entry.
-void plan_unused(Route &p, const int32_t *source) {
-  p.unused_rows = unused_rows_of(p.rows);
+void plan_unused(Route &p, const int32_t *source, int elem_bytes) {
+  p.unused_rows = unused_rows_of(p.rows, (uint64_t)p.tokens * p.slots, (uint64_t)p.width * elem_bytes);
   const uint32_t block = p.unused_rows * (kRowThreads / 32);
   p.unused_blocks = source ? (p.rows + block - 1) / block : 0;
 }
 
 // The grid of the kernels whose threads take a vector of a token's row.
-dim3 token_grid(Route &p, const int32_t *source, bool whole_warps) {
+dim3 token_grid(Route &p, const int32_t *source, int elem_bytes, bool whole_warps) {
   p.flat = flat_tokens(p.tokens, p.vectors, whole_warps);
-  plan_unused(p, source);
+  plan_unused(p, source, elem_bytes);
   return dim3(p.flat.grid.x + p.unused_blocks, std::max(1u, p.flat.grid.y));
 }
 
@@ -433,7 +445,7 @@ int dcopy_expert_dispatch(const DcopyMatrix *out, const DcopyMatrix *x, const in
       constexpr int kFull = 16 / sizeof(T), kLeast = 8 / sizeof(T);
       const Cut cut = cut_rows(kFull, kLeast, out, x);
       p.vectors = vectors_of(out->cols, cut);
-      const dim3 grid = token_grid(p, source, true);
+      const dim3 grid = token_grid(p, source, sizeof(T), true);
       if (grid.x == 0) return (int)DCOPY_OK;
       return with_cut<kFull, kLeast>(cut, [&](auto v, auto shift) {
         return launch_grid(dispatch_weighted_kernel<T, v(), shift()>, grid, dim3(kRowThreads), 0,
@@ -452,7 +464,7 @@ int dcopy_expert_dispatch(const DcopyMatrix *out, const DcopyMatrix *x, const in
   // shifted).
   const Cut cut = all % 16 == 0 ? Cut{16, false} : all % 8 == 0 ? Cut{8, false} : Cut{16, true};
   p.vectors = vectors_of(p.width, cut);
-  const dim3 grid = token_grid(p, source, true);
+  const dim3 grid = token_grid(p, source, 1, true);
   if (grid.x == 0) return DCOPY_OK;
   auto k = cut.shift ? dispatch_shift_kernel : cut.v == 16 ? dispatch_kernel<16> : dispatch_kernel<8>;
   return launch_grid(k, grid, dim3(kRowThreads), 0, stream, "dispatch_kernel", p);
@@ -490,7 +502,7 @@ int dcopy_expert_combine(const DcopyMatrix *out, const DcopyMatrix *y, const int
     constexpr int kFull = 16 / sizeof(T), kLeast = 4 / sizeof(T);
     const Cut cut = cut_rows(kFull, kLeast, out, y);
     p.vectors = vectors_of(out->cols, cut);
-    const dim3 grid = token_grid(p, nullptr, false);
+    const dim3 grid = token_grid(p, nullptr, sizeof(T), false);
     return with_cut<kFull, kLeast>(cut, [&](auto v, auto shift) {
       return launch_grid(combine_kernel<T, v(), shift()>, grid, dim3(kRowThreads), 0, stream,
                          "combine_kernel", p);
@@ -538,11 +550,10 @@ int dcopy_expert_combine_grad(const DcopyMatrix *dy, const DcopyMatrix *dweights
   p.tokens = (uint32_t)dout->rows;
   p.slots = (uint32_t)slots;
   p.rows = (uint32_t)dy->rows;
-  plan_unused(p, source);
+  p.width = (uint32_t)dy->cols;
+  plan_unused(p, source, elem_size(dy->type));
   p.by_slots = FastDiv((uint32_t)std::max<int64_t>(1, slots));
   const uint64_t entries = (uint64_t)p.tokens * p.slots;
-  p.width = (uint32_t)dy->cols;
-  p.width = (uint32_t)dy->cols;
   return with_float(dy->type, [&](auto t) {
     using T = typename decltype(t)::type;
     // Never shifted: 24390 x 4 entries of 1025 bf16 take 138 us in single elements, 182
@@ -552,6 +563,9 @@ int dcopy_expert_combine_grad(const DcopyMatrix *dy, const DcopyMatrix *dweights
     p.vectors = vectors_of(dy->cols, cut);
     p.lx = 0;
     while (p.lx < 5 && (1u << p.lx) < p.vectors) ++p.lx;
+    // A block an entry where warps alone would leave SMs idle (13 x 6 entries of 8192 fp32:
+    // 4.6 us against 9.4; 600 x 4 of 2048 bf16: 6.0 against 8.4; 1000 x 4: 13.1 against 6.4).
+    if (p.vectors >= 128 && entries <= 16ull * sm_count()) p.lx = 8;
     const uint64_t per_block = kRowThreads >> p.lx;
     const uint64_t blocks = p.unused_blocks + (entries + per_block - 1) / per_block;
     if (blocks == 0) return (int)DCOPY_OK;
