@@ -368,6 +368,39 @@ PyObject *clip_grad_norm(PyObject *, PyObject *const *a, Py_ssize_t n) {
   });
 }
 
+// fill_grads(address, grads, outs) -> device: DcopyGrad records of two lists of tensors.
+PyObject *fill_grads(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  try {
+    if (n != 3 || !PyList_Check(a[1]) || !PyList_Check(a[2]))
+      value_error("fill_grads", "expected an address and two lists");
+    auto *record = reinterpret_cast<DcopyGrad *>((uintptr_t)as_int(a[0]));
+    const Py_ssize_t count = PyList_Size(a[1]);
+    if (PyList_Size(a[2]) != count) value_error("out", "needs a tensor for each gradient");
+    int64_t device = -1;
+    for (Py_ssize_t i = 0; i < count; ++i) {
+      const at::Tensor &g = unpack(PyList_GetItem(a[1], i), "gradient");
+      const at::Tensor &o = unpack(PyList_GetItem(a[2], i), "out");
+      const std::string name = "gradient " + std::to_string(i);
+      if (!g.is_cuda() || !o.is_cuda() || !g.is_contiguous() || !o.is_contiguous())
+        value_error(name.c_str(), "expected contiguous CUDA tensors");
+      if (g.numel() != o.numel())
+        value_error(name.c_str(), std::to_string(g.numel()) + " elements for " +
+                                      std::to_string(o.numel()));
+      if (device < 0) device = g.get_device();
+      if (g.get_device() != device || o.get_device() != device)
+        value_error(name.c_str(), "tensors are on different devices");
+      record[i] = DcopyGrad{g.const_data_ptr(), const_cast<void *>(o.const_data_ptr()),
+                            (uint64_t)g.numel(), type_code(g.scalar_type()),
+                            type_code(o.scalar_type())};
+    }
+    return PyLong_FromLongLong(device);
+  } catch (const Raised &) {
+  } catch (const std::exception &e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+  }
+  return nullptr;
+}
+
 // layout(tensor) -> (rows, cols, pitch, type): how a call sees a tensor, on any device.
 PyObject *layout_of(PyObject *, PyObject *o) {
   try {
@@ -406,7 +439,7 @@ PyObject *bind(PyObject *, PyObject *args) {
 PyMethodDef methods[] = {
     FAST(embedding_lookup), FAST(embedding_grad), FAST(expert_sort), FAST(expert_dispatch),
     FAST(expert_combine), FAST(expert_combine_grad), FAST(grad_sum_squares), FAST(grad_clip),
-    FAST(clip_grad_norm),
+    FAST(clip_grad_norm), FAST(fill_grads),
     {"layout", layout_of, METH_O, nullptr},
     {"bind", bind, METH_VARARGS, nullptr},
     {nullptr, nullptr, 0, nullptr}};

@@ -343,6 +343,7 @@ int dcopy_grad_list_build(DcopyGradList *list, const DcopyGrad *grads, uint32_t 
     if (g.src != g.dst || g.src_type != g.dst_type)  // in place, or apart
       if (int rc = check_disjoint(g.src, g.count * sb, g.dst, g.count * db, "gradient")) return rc;
     // The first chunk takes the head too; the others start on a vector.
+    std::vector<Chunk> &mine = chunks[3 * type_index(g.src_type) + type_index(g.dst_type)];
     const uint64_t head = head_of(g);
     const bool scalar = head == g.count;
     for (uint64_t at = 0; at < g.count;) {
@@ -352,7 +353,7 @@ int dcopy_grad_list_build(DcopyGradList *list, const DcopyGrad *grads, uint32_t 
       c.dst = static_cast<uint8_t *>(g.dst) + at * db;
       c.count = (uint32_t)std::min<uint64_t>(most, g.count - at);
       c.head = scalar ? c.count : at == 0 ? (uint32_t)head : 0;
-      chunks[3 * type_index(g.src_type) + type_index(g.dst_type)].push_back(c);
+      mine.push_back(c);
       at += c.count;
     }
   }

@@ -132,25 +132,14 @@ class GradList:
         import torch
         grads = list(grads)
         out = grads if out is None else list(out)
-        if len(grads) != len(out):
-            raise ValueError("out needs a tensor for each gradient")
         if not grads:
             raise ValueError("no gradients")
         arr = (DcopyGrad * len(grads))()
-        for k, (g, o) in enumerate(zip(grads, out)):
-            if not (g.is_cuda and o.is_cuda and g.is_contiguous() and o.is_contiguous()):
-                raise ValueError(f"gradient {k}: expected contiguous CUDA tensors")
-            if g.numel() != o.numel():
-                raise ValueError(f"gradient {k}: {g.numel()} elements for {o.numel()}")
-            if g.device != grads[0].device or o.device != grads[0].device:
-                raise ValueError("tensors are on different devices")
-            arr[k] = DcopyGrad(g.data_ptr(), o.data_ptr(), g.numel(), _calls.layout(g)[3],
-                               _calls.layout(o)[3])
+        self._device = _calls.fill_grads(ctypes.addressof(arr), grads, out)
         n = ctypes.c_uint64(0)
         _check(lib().dcopy_grad_list_workspace(arr, len(arr), ctypes.byref(n)),
                "dcopy_grad_list_workspace")
         self._tensors = (grads, out)
-        self._device = grads[0].get_device()
         self._list = DcopyGradList()
         self._address = ctypes.addressof(self._list)
         with torch.cuda.device(self._device):
