@@ -509,7 +509,8 @@ int dcopy_memcpy_async_batch(const DcopyMemcpyInfo *infos, uint32_t count, int32
  * Operators of language models that move or sum rows picked by index.  The
  * reference has no counterpart.  Elements are FLOAT (0), FLOAT16 (1) or BF16 (27);
  * sums are held in fp32 and rounded once, to nearest even.  Every result is the
- * same on every run: no sum depends on the order in which blocks execute. */
+ * same on every run: no sum depends on the order in which blocks execute.  Widths
+ * beyond 2^23 are UNSUPPORTED, rows and ids beyond 2^31 - 1 SHAPE_INVALID. */
 
 /* rows x cols elements of a GE DataType, rows `pitch` elements apart (at least
  * cols; not looked at when rows <= 1).  data is aligned to the element. */
