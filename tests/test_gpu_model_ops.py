@@ -285,6 +285,33 @@ def test_expert_sort_of_few_and_odd_choices(torch_cuda, dcopy):
         assert np.array_equal(offsets.cpu().numpy(), o)
 
 
+def test_sorts_of_millions(torch_cuda, dcopy):
+    """Lists beyond the smaller tiles of the sort: 5 M choices and 4.3 M tokens."""
+    g = gen(17)
+    ids = torch.randint(-1, 38, (2500000, 2), generator=g, device="cuda")
+    dest, source, offsets = sorted_route(dcopy, ids, (2500000, 2, 37, 3, 0.0))
+    flat = ids.view(-1)
+    key = torch.where((flat >= 0) & (flat < 37), flat, 37)
+    order = torch.argsort(key, stable=True)
+    count = torch.bincount(key, minlength=38)
+    first, padded = torch.cumsum(count, 0) - count, (count[:37] + 2) // 3 * 3
+    ends = torch.cat([padded.new_zeros(1), torch.cumsum(padded, 0)])
+    assert torch.equal(offsets.long(), ends)
+    row = torch.arange(flat.numel(), device="cuda") - first[key[order]] + ends[key[order]]
+    row = torch.where(key[order] < 37, row, -1)
+    assert torch.equal(dest.view(-1)[order].long(), row)
+    want = torch.full_like(source, -1)
+    want[row[row >= 0]] = order[row >= 0].int()
+    assert torch.equal(source, want)
+    tokens, vocab = 4300000, 3001
+    ids = torch.randint(-1, vocab + 1, (tokens,), generator=g, device="cuda", dtype=torch.int32)
+    dout = randn(g, (tokens, 4), F32)
+    grad = torch.empty(vocab, 4, device="cuda")
+    dcopy.embedding_grad(grad, dout, ids)
+    exact, size = grad_exact(dout, ids.long(), vocab, 1.0)
+    close(grad, exact, int(torch.bincount(ids.clamp(0, vocab - 1)).max()), size)
+
+
 WIDTHS = [(1, 0, 0), (8, 0, 0), (17, 3, 5), (100, 4, 0), (257, 1, 1), (1024, 0, 0), (1030, 0, 0),
           (2056, 8, 8)]
 
