@@ -10,7 +10,6 @@
 
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
-#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -140,7 +139,8 @@ class Call {
   }
   void on_device(int64_t device) { device_ = device; }
 
-  // Fixes device and stream; after the tensors were read.
+  // Fixes device and stream; after the tensors were read.  A given stream is torch's
+  // current one for the rest of the call.
   dcopy_stream_t stream() {
     guard_.emplace((c10::DeviceIndex)device_);
     if (given_ == Py_None)
@@ -152,10 +152,13 @@ class Call {
     const unsigned long long raw = PyLong_AsUnsignedLongLong(value);
     Py_DECREF(value);
     if (PyErr_Occurred()) throw Raised{};
-    return reinterpret_cast<dcopy_stream_t>((uintptr_t)raw);
+    const auto s = reinterpret_cast<cudaStream_t>((uintptr_t)raw);
+    on_stream_.emplace(c10::cuda::getStreamFromExternal(s, (c10::DeviceIndex)device_));
+    return reinterpret_cast<dcopy_stream_t>(s);
   }
-  // The given workspace, or one from the allocator that is kept until `s` is done.
-  void *workspace(PyObject *o, uint64_t need, dcopy_stream_t s, uint64_t *bytes) {
+  // The given workspace, or one from the allocator: of the pool of the call's stream, so
+  // that neither a block's last user nor its next can meet the call's kernels.
+  void *workspace(PyObject *o, uint64_t need, uint64_t *bytes) {
     if (o != Py_None) {
       const at::Tensor &t = tensor(o, "workspace");
       if (!t.is_contiguous()) value_error("workspace", "expected a contiguous tensor");
@@ -164,10 +167,6 @@ class Call {
     }
     scratch_ = at::empty({(int64_t)need}, at::TensorOptions().dtype(at::kByte).device(
                                               at::Device(at::kCUDA, (c10::DeviceIndex)device_)));
-    const auto ext = c10::cuda::getStreamFromExternal(reinterpret_cast<cudaStream_t>(s),
-                                                      (c10::DeviceIndex)device_);
-    if (given_ != Py_None)
-      c10::cuda::CUDACachingAllocator::recordStream(scratch_.storage().data_ptr(), ext);
     *bytes = need;
     return scratch_.mutable_data_ptr();
   }
@@ -181,6 +180,7 @@ class Call {
   PyObject *given_;
   int64_t device_ = -1;
   std::optional<c10::cuda::CUDAGuard> guard_;
+  std::optional<c10::cuda::CUDAStreamGuard> on_stream_;
   at::Tensor scratch_;
 };
 
@@ -240,7 +240,7 @@ PyObject *embedding_grad(PyObject *, PyObject *const *a, Py_ssize_t n) {
     uint64_t need = 0, bytes = 0;
     if (a[6] == Py_None)
       c.check(lib.dcopy_embedding_grad_workspace(ids.rows * ids.cols, grad.rows, grad.cols, &need));
-    void *space = c.workspace(a[6], need, s, &bytes);
+    void *space = c.workspace(a[6], need, &bytes);
     c.check(unlocked([&] {
       return lib.dcopy_embedding_grad(&grad, &dout, &ids, first, scale, accumulate, space, bytes, s);
     }));
@@ -261,7 +261,7 @@ PyObject *expert_sort(PyObject *, PyObject *const *a, Py_ssize_t n) {
     dcopy_stream_t s = c.stream();
     uint64_t need = 0, bytes = 0;
     if (a[5] == Py_None) c.check(lib.dcopy_expert_sort_workspace(entries, experts, &need));
-    void *space = c.workspace(a[5], need, s, &bytes);
+    void *space = c.workspace(a[5], need, &bytes);
     c.check(unlocked([&] {
       return lib.dcopy_expert_sort(dest, source, rows, offsets, &ids, experts, align, space, bytes, s);
     }));
