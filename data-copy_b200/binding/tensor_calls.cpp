@@ -10,6 +10,7 @@
 
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -152,9 +153,13 @@ class Call {
     const unsigned long long raw = PyLong_AsUnsignedLongLong(value);
     Py_DECREF(value);
     if (PyErr_Occurred()) throw Raised{};
-    const auto s = reinterpret_cast<cudaStream_t>((uintptr_t)raw);
-    on_stream_.emplace(c10::cuda::getStreamFromExternal(s, (c10::DeviceIndex)device_));
-    return reinterpret_cast<dcopy_stream_t>(s);
+    const auto s = reinterpret_cast<dcopy_stream_t>((uintptr_t)raw);
+    on_stream_.emplace(torch_stream(s));
+    return s;
+  }
+  c10::cuda::CUDAStream torch_stream(dcopy_stream_t s) const {
+    return c10::cuda::getStreamFromExternal(reinterpret_cast<cudaStream_t>(s),
+                                            (c10::DeviceIndex)device_);
   }
   // The given workspace, or one from the allocator: of the pool of the call's stream, so
   // that neither a block's last user nor its next can meet the call's kernels.
@@ -170,6 +175,7 @@ class Call {
     *bytes = need;
     return scratch_.mutable_data_ptr();
   }
+  const at::Tensor &taken() const { return scratch_; }
   void check(int rc) {
     if (rc) dcopy_error(rc, lib.dcopy_last_error_message(), func_);
   }
@@ -332,40 +338,89 @@ PyObject *expert_combine_grad(PyObject *, PyObject *const *a, Py_ssize_t n) {
   });
 }
 
-// (address of the DcopyGradList, device, ...)
-const DcopyGradList *grad_list(Call &c, PyObject *address, PyObject *device) {
-  c.on_device(as_int(device));
-  return reinterpret_cast<const DcopyGradList *>((uintptr_t)as_int(address));
+// A list of gradients as Python holds it: (address of the DcopyGradList, device, the tensors
+// that it keeps, the streams they are known to be used on).
+struct Gradients {
+  const DcopyGradList *list;
+  PyObject *tensors, *streams;
+};
+Gradients gradients(Call &c, PyObject *o) {
+  if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 4 || !PyList_Check(PyTuple_GET_ITEM(o, 2)) ||
+      !PySet_Check(PyTuple_GET_ITEM(o, 3)))
+    value_error("gradients", "expected a GradList");
+  c.on_device(as_int(PyTuple_GET_ITEM(o, 1)));
+  return {reinterpret_cast<const DcopyGradList *>((uintptr_t)as_int(PyTuple_GET_ITEM(o, 0))),
+          PyTuple_GET_ITEM(o, 2), PyTuple_GET_ITEM(o, 3)};
+}
+
+// Tells the allocator of a list's first use on a stream: its memory, should the list be
+// dropped, waits for what that stream holds by then.
+void use_on(const Gradients &g, Call &c, dcopy_stream_t s) {
+  PyObject *key = PyLong_FromVoidPtr(s);
+  const int known = key ? PySet_Contains(g.streams, key) : -1;
+  if (known == 0) {
+    const auto stream = c.torch_stream(s);
+    for (Py_ssize_t i = 0; i < PyList_GET_SIZE(g.tensors); ++i)
+      c10::cuda::CUDACachingAllocator::recordStream(
+          unpack(PyList_GET_ITEM(g.tensors, i), "gradient").storage().data_ptr(), stream);
+  }
+  const bool failed = known < 0 || (known == 0 && PySet_Add(g.streams, key));
+  Py_XDECREF(key);
+  if (failed) throw Raised{};
 }
 
 PyObject *grad_sum_squares(PyObject *, PyObject *const *a, Py_ssize_t n) {
-  return run("dcopy_grad_sum_squares", a, n, 4, [&](Call &c) {
-    const DcopyGradList *list = grad_list(c, a[0], a[1]);
-    auto *total = (double *)c.vector(a[2], "total", at::kDouble);
+  return run("dcopy_grad_sum_squares", a, n, 3, [&](Call &c) {
+    const Gradients g = gradients(c, a[0]);
+    auto *total = (double *)c.vector(a[1], "total", at::kDouble);
     dcopy_stream_t s = c.stream();
-    c.check(unlocked([&] { return lib.dcopy_grad_sum_squares(list, total, s); }));
+    use_on(g, c, s);
+    c.check(unlocked([&] { return lib.dcopy_grad_sum_squares(g.list, total, s); }));
   });
 }
 
 PyObject *grad_clip(PyObject *, PyObject *const *a, Py_ssize_t n) {
-  return run("dcopy_grad_clip", a, n, 7, [&](Call &c) {
-    const DcopyGradList *list = grad_list(c, a[0], a[1]);
-    auto *total = (const double *)c.vector(a[2], "total", at::kDouble);
-    const float max_norm = (float)as_double(a[3]), eps = (float)as_double(a[4]);
-    auto *norm = (float *)c.vector(a[5], "norm", at::kFloat);
+  return run("dcopy_grad_clip", a, n, 6, [&](Call &c) {
+    const Gradients g = gradients(c, a[0]);
+    auto *total = (const double *)c.vector(a[1], "total", at::kDouble);
+    const float max_norm = (float)as_double(a[2]), eps = (float)as_double(a[3]);
+    auto *norm = (float *)c.vector(a[4], "norm", at::kFloat);
     dcopy_stream_t s = c.stream();
-    c.check(unlocked([&] { return lib.dcopy_grad_clip(list, total, max_norm, eps, norm, s); }));
+    use_on(g, c, s);
+    c.check(unlocked([&] { return lib.dcopy_grad_clip(g.list, total, max_norm, eps, norm, s); }));
   });
 }
 
 PyObject *clip_grad_norm(PyObject *, PyObject *const *a, Py_ssize_t n) {
-  return run("dcopy_clip_grad_norm", a, n, 6, [&](Call &c) {
-    const DcopyGradList *list = grad_list(c, a[0], a[1]);
-    const float max_norm = (float)as_double(a[2]), eps = (float)as_double(a[3]);
-    auto *norm = (float *)c.vector(a[4], "norm", at::kFloat);
+  return run("dcopy_clip_grad_norm", a, n, 5, [&](Call &c) {
+    const Gradients g = gradients(c, a[0]);
+    const float max_norm = (float)as_double(a[1]), eps = (float)as_double(a[2]);
+    auto *norm = (float *)c.vector(a[3], "norm", at::kFloat);
     dcopy_stream_t s = c.stream();
-    c.check(unlocked([&] { return lib.dcopy_clip_grad_norm(list, max_norm, eps, norm, s); }));
+    use_on(g, c, s);
+    c.check(unlocked([&] { return lib.dcopy_clip_grad_norm(g.list, max_norm, eps, norm, s); }));
   });
+}
+
+// scratch(bytes, device, stream) -> (tensor, the stream's handle): memory of that stream's
+// pool, by default the current one's.
+PyObject *scratch(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  if (n != 3) {
+    PyErr_SetString(PyExc_TypeError, "scratch takes 3 arguments");
+    return nullptr;
+  }
+  try {
+    Call c("scratch", a[2]);
+    c.on_device(as_int(a[1]));
+    dcopy_stream_t s = c.stream();
+    uint64_t bytes = 0;
+    c.workspace(Py_None, (uint64_t)as_int(a[0]), &bytes);
+    return Py_BuildValue("NN", THPVariable_Wrap(c.taken()), PyLong_FromVoidPtr(s));
+  } catch (const Raised &) {
+  } catch (const std::exception &e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+  }
+  return nullptr;
 }
 
 // fill_grads(address, grads, outs) -> device: DcopyGrad records of two lists of tensors.
@@ -439,7 +494,7 @@ PyObject *bind(PyObject *, PyObject *args) {
 PyMethodDef methods[] = {
     FAST(embedding_lookup), FAST(embedding_grad), FAST(expert_sort), FAST(expert_dispatch),
     FAST(expert_combine), FAST(expert_combine_grad), FAST(grad_sum_squares), FAST(grad_clip),
-    FAST(clip_grad_norm), FAST(fill_grads),
+    FAST(clip_grad_norm), FAST(fill_grads), FAST(scratch),
     {"layout", layout_of, METH_O, nullptr},
     {"bind", bind, METH_VARARGS, nullptr},
     {nullptr, nullptr, 0, nullptr}};

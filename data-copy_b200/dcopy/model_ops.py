@@ -21,7 +21,7 @@ from __future__ import annotations
 import ctypes
 from typing import Sequence
 
-from . import DcopyError, DcopyGrad, DcopyGradList, DcopyUnavailable, _check, _stream, lib
+from . import DcopyError, DcopyGrad, DcopyGradList, DcopyUnavailable, _check, lib
 
 __all__ = ["embedding_lookup", "embedding_grad", "embedding_grad_workspace", "expert_rows",
            "expert_sort", "expert_sort_workspace", "expert_dispatch", "expert_combine",
@@ -126,7 +126,10 @@ class GradList:
     ``grads`` are dense CUDA tensors (FLOAT, FLOAT16 or BF16, mixed as they come); clipped
     values go to ``out`` (same sizes, any of the types), by default in place.  The list keeps
     the tensors alive; gradients that move to other buffers need a new list.  Uses of one list
-    follow one another on a stream.  Building it synchronises."""
+    follow one another on a stream.  Building it synchronises.
+
+    A list may be dropped while its last use still runs, on any stream: the memory that it
+    held is not handed out before the streams it was used on are done with it."""
 
     def __init__(self, grads: Sequence, out: Sequence = None, stream=None):
         import torch
@@ -135,32 +138,32 @@ class GradList:
         if not grads:
             raise ValueError("no gradients")
         arr = (DcopyGrad * len(grads))()
-        self._device = _calls.fill_grads(ctypes.addressof(arr), grads, out)
+        device = _calls.fill_grads(ctypes.addressof(arr), grads, out)
         n = ctypes.c_uint64(0)
         _check(lib().dcopy_grad_list_workspace(arr, len(arr), ctypes.byref(n)),
                "dcopy_grad_list_workspace")
-        self._tensors = (grads, out)
         self._list = DcopyGradList()
-        self._address = ctypes.addressof(self._list)
-        with torch.cuda.device(self._device):
-            self._space = torch.empty(n.value, dtype=torch.uint8, device="cuda")
+        self._space, handle = _calls.scratch(n.value, device, stream)
+        with torch.cuda.device(device):
             _check(lib().dcopy_grad_list_build(ctypes.byref(self._list), arr, len(arr),
-                                               self._space.data_ptr(), n.value, _stream(stream)),
+                                               self._space.data_ptr(), n.value, handle),
                    "dcopy_grad_list_build")
+        kept = [self._space] + grads + (out if out is not grads else [])
+        self._record = (ctypes.addressof(self._list), device, kept, {handle})
 
 
 def grad_sum_squares(total, grads: GradList, stream=None) -> None:
     """total[0] (fp64, CUDA) = the sum of squares over the list."""
-    _calls.grad_sum_squares(grads._address, grads._device, total, stream)
+    _calls.grad_sum_squares(grads._record, total, stream)
 
 
 def grad_clip(grads: GradList, total, max_norm: float, norm=None, eps: float = 1e-6,
               stream=None) -> None:
     """Clips the list by the norm sqrt(total[0]); norm[0] (fp32, CUDA) gets it."""
-    _calls.grad_clip(grads._address, grads._device, total, max_norm, eps, norm, stream)
+    _calls.grad_clip(grads._record, total, max_norm, eps, norm, stream)
 
 
 def clip_grad_norm(grads: GradList, max_norm: float, norm=None, eps: float = 1e-6,
                    stream=None) -> None:
     """The list times min(1, max_norm / (norm + eps)); norm[0] (fp32, CUDA) gets the norm."""
-    _calls.clip_grad_norm(grads._address, grads._device, max_norm, eps, norm, stream)
+    _calls.clip_grad_norm(grads._record, max_norm, eps, norm, stream)

@@ -66,3 +66,69 @@ def test_workspaces_are_the_given_streams(dcopy, fresh_stream, as_number):
     got = [t.clone() for t in outs]
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+def span(t):
+    return t.data_ptr(), t.data_ptr() + t.nbytes
+
+
+@pytest.mark.parametrize("given", ["stream", "number", "current"])
+@pytest.mark.parametrize("call", ["clip_grad_norm", "grad_sum_squares", "grad_clip"])
+def test_a_dropped_list_is_kept_until_its_streams_are_done(torch_cuda, dcopy, given, call):
+    """A list dropped while another stream's call on it is still pending: the memory of its
+    table, and of outputs that only the list held, goes to nobody else before."""
+    side = torch.cuda.Stream()
+    g = torch.Generator(device="cuda").manual_seed(5)
+    grads = [torch.randn(n, generator=g, device="cuda") for n in (100003, 7, 4096, 50000)]
+    want = [t.clone() for t in grads]
+    norm, total = torch.empty(1, device="cuda"), torch.empty(1, dtype=torch.float64, device="cuda")
+    args = {"clip_grad_norm": (1.0, norm), "grad_clip": (total, 1.0, norm)}.get(call)
+
+    def run(grads, outs, **stream):
+        held = dcopy.GradList(grads, outs)
+        if call == "grad_sum_squares":
+            dcopy.grad_sum_squares(total, held, **stream)
+        else:
+            dcopy.__dict__[call](held, *args, **stream)
+        return held
+
+    total.fill_(9.0)
+    run(want, None)
+    torch.cuda.synchronize()
+    expected = float(total if call == "grad_sum_squares" else norm)
+    norm.zero_()
+    if call == "grad_sum_squares":
+        total.zero_()
+    outs = [torch.empty_like(t) for t in grads]
+    for t in grads:
+        t.record_stream(side)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(5 * BUSY)
+    if given == "current":
+        held = dcopy.GradList(grads, outs)
+        with torch.cuda.stream(side):
+            if call == "grad_sum_squares":
+                dcopy.grad_sum_squares(total, held)
+            else:
+                dcopy.__dict__[call](held, *args)
+    else:
+        held = run(grads, outs, stream=side if given == "stream" else side.cuda_stream)
+    kept = [held._space] + outs
+    taken, sizes = [span(t) for t in kept], [t.nbytes for t in kept]
+    del kept, held, outs
+    others = [torch.empty(n, dtype=torch.uint8, device="cuda") for n in sizes for _ in range(8)]
+    assert not side.query()  # still busy
+    assert all(b <= lo or hi <= a for a, b in taken for lo, hi in map(span, others))
+    side.synchronize()
+    assert float(total if call == "grad_sum_squares" else norm) == expected
+
+
+def test_a_list_lives_on_the_stream_it_is_built_on(dcopy, fresh_stream):
+    """The table's memory is of the given stream's pool, as the copy that fills it runs there."""
+    grads = [torch.ones(1000, device="cuda")]
+    held = dcopy.GradList(grads, stream=fresh_stream)
+    assert pool_bytes(fresh_stream) >= held._space.nbytes
+    norm = torch.empty(1, device="cuda")
+    dcopy.clip_grad_norm(held, 1.0, norm)
+    assert abs(norm.item() - 1000 ** 0.5) <= 40 * 2.0 ** -24 * 1000 ** 0.5
