@@ -283,12 +283,14 @@ def _embedding_backward_fake(dout, ids, vocab, scale=1.0, first_id=0):
 
 
 def _embedding_setup(ctx, inputs, output):
-    table, ctx.ids, ctx.scale, ctx.first_id = inputs
+    table, ids, ctx.scale, ctx.first_id = inputs
     ctx.vocab = table.shape[0]
+    ctx.save_for_backward(ids)
 
 
 def _embedding_grad(ctx, dout):
-    return embedding_backward(dout, ctx.ids, ctx.vocab, ctx.scale, ctx.first_id), None, None, None
+    ids, = ctx.saved_tensors
+    return embedding_backward(dout, ids, ctx.vocab, ctx.scale, ctx.first_id), None, None, None
 
 
 embedding.register_autograd(_embedding_grad, setup_context=_embedding_setup)
@@ -355,27 +357,29 @@ def _expert_combine_backward_fake(dout, y, dest, source, weights):
 
 
 def _dispatch_setup(ctx, inputs, output):
-    _, ctx.dest, ctx.source = inputs
+    _, dest, source = inputs
+    ctx.save_for_backward(dest, source)
 
 
 def _dispatch_grad(ctx, dout):
-    return expert_combine(dout, ctx.dest, ctx.source, None), None, None
+    dest, source = ctx.saved_tensors
+    return expert_combine(dout, dest, source, None), None, None
 
 
 expert_dispatch.register_autograd(_dispatch_grad, setup_context=_dispatch_setup)
 
 
 def _combine_setup(ctx, inputs, output):
-    y, ctx.dest, ctx.source, weights = inputs
+    y, dest, source, weights = inputs
     ctx.weighted = weights is not None
-    ctx.save_for_backward(*((y, weights) if ctx.weighted else ()))
+    ctx.save_for_backward(dest, source, *((y, weights) if ctx.weighted else ()))
 
 
 def _combine_grad(ctx, dout):
+    dest, source, *weighted = ctx.saved_tensors
     if not ctx.weighted:
-        return expert_dispatch(dout, ctx.dest, ctx.source), None, None, None
-    dy, dweights = expert_combine_backward(dout, ctx.saved_tensors[0], ctx.dest, ctx.source,
-                                           ctx.saved_tensors[1])
+        return expert_dispatch(dout, dest, source), None, None, None
+    dy, dweights = expert_combine_backward(dout, weighted[0], dest, source, weighted[1])
     return dy, None, None, dweights
 
 
