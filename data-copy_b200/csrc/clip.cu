@@ -10,6 +10,7 @@
 
 #include <algorithm>
 #include <cstring>
+#include <string>
 #include <vector>
 
 #include "common.cuh"
@@ -233,6 +234,35 @@ int check_grads(const DcopyGrad *grads, uint32_t n, const char *what) {
   return DCOPY_OK;
 }
 
+// Memory that a list reads or writes, and the gradient it belongs to.
+struct Span {
+  uintptr_t begin, end;
+  uint32_t gradient;
+  bool written;
+};
+constexpr uint32_t kSpanOfWorkspace = UINT32_MAX;
+
+std::string name_of(const Span &s) {
+  if (s.gradient == kSpanOfWorkspace) return "the workspace";
+  return (s.written ? "the output of gradient " : "gradient ") + std::to_string(s.gradient);
+}
+
+// What is written meets nothing else: the chunks of a list run in any order.
+int check_spans(std::vector<Span> &spans) {
+  std::sort(spans.begin(), spans.end(),
+            [](const Span &a, const Span &b) { return a.begin < b.begin; });
+  const Span *furthest = nullptr, *written = nullptr;  // of those before, by their ends
+  for (const Span &s : spans) {
+    const Span *other = s.written ? furthest : written;
+    if (other && s.begin < other->end)
+      return set_error(DCOPY_ERR_PARAM_INVALID, "%s overlaps %s", name_of(s).c_str(),
+                       name_of(*other).c_str());
+    if (!furthest || s.end > furthest->end) furthest = &s;
+    if (s.written && (!written || s.end > written->end)) written = &s;
+  }
+  return DCOPY_OK;
+}
+
 int open_list(const DcopyGradList *list) {
   if (!list || !list->workspace)
     return set_error(DCOPY_ERR_PARAM_INVALID, "gradient list: not built");
@@ -329,6 +359,7 @@ int dcopy_grad_list_build(DcopyGradList *list, const DcopyGrad *grads, uint32_t 
                      (unsigned long long)workspace_bytes, workspace, (unsigned long long)need);
   if (int rc = check_device_span(workspace, need, "workspace")) return rc;
   std::vector<Chunk> chunks[kPairs];
+  std::vector<Span> spans{{(uintptr_t)workspace, (uintptr_t)workspace + need, kSpanOfWorkspace, true}};
   for (uint32_t i = 0; i < n; ++i) {
     const DcopyGrad &g = grads[i];
     if (!is_float(g.src_type) || !is_float(g.dst_type))
@@ -340,8 +371,9 @@ int dcopy_grad_list_build(DcopyGradList *list, const DcopyGrad *grads, uint32_t 
       return set_error(DCOPY_ERR_PARAM_INVALID, "gradient %u is not aligned to its elements", i);
     if (int rc = check_device_span(g.src, g.count * sb, "gradient")) return rc;
     if (int rc = check_device_span(g.dst, g.count * db, "clipped gradient")) return rc;
-    if (g.src != g.dst || g.src_type != g.dst_type)  // in place, or apart
-      if (int rc = check_disjoint(g.src, g.count * sb, g.dst, g.count * db, "gradient")) return rc;
+    if (g.src != g.dst || g.src_type != g.dst_type)  // else in place
+      spans.push_back({(uintptr_t)g.src, (uintptr_t)g.src + g.count * sb, i, false});
+    spans.push_back({(uintptr_t)g.dst, (uintptr_t)g.dst + g.count * db, i, true});
     // The first chunk takes the head too; the others start on a vector.
     std::vector<Chunk> &mine = chunks[3 * type_index(g.src_type) + type_index(g.dst_type)];
     const uint64_t head = head_of(g);
@@ -357,6 +389,7 @@ int dcopy_grad_list_build(DcopyGradList *list, const DcopyGrad *grads, uint32_t 
       at += c.count;
     }
   }
+  if (int rc = check_spans(spans)) return rc;
   list->workspace = workspace;
   list->first[0] = 0;
   for (int q = 0; q < kPairs; ++q) {

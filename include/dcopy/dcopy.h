@@ -574,7 +574,8 @@ int dcopy_expert_combine_grad(const DcopyMatrix *dy, const DcopyMatrix *dweights
                               dcopy_stream_t stream);
 
 /* One gradient of a list: count elements from src, clipped into dst (src itself for
- * in place, else apart from it). */
+ * in place).  What is written overlaps nothing else of the list, be it a gradient, an
+ * output or the workspace. */
 typedef struct DcopyGrad {
   const void *src;
   void *dst;

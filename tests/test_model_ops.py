@@ -117,3 +117,29 @@ def test_records_match_the_c_abi(dcopy, tmp_path, monkeypatch):
         "DcopyGradList": ["workspace", "first"],
     })
     layout.test_ctypes_records_match_the_c_abi(dcopy, tmp_path)
+
+
+@pytest.mark.parametrize("spans,fine", [
+    ([(0, 0), (400, 400)], True), ([(0, 1000), (400, 1400)], True),
+    ([(0, 1000), (0, 2000)], True),           # one gradient, clipped into two places
+    ([(0, 0), (0, 0)], False),                # one gradient twice in place
+    ([(0, 0), (396, 396)], False), ([(396, 396), (0, 0)], False),
+    ([(0, 1000), (1000, 2000)], False),       # an output is the next gradient
+    ([(0, 1000), (400, 1004)], False),        # two outputs meet
+    ([(0, 1000), (400, 2000), (2396, 3000)], False),
+    ([(0, 4)], False),                        # neither in place nor apart
+    ([(0, 20000)], False),                    # the output is the workspace
+    ([(100000 - 400, 0)], True), ([(0, 4000), (4, 8000), (8, 12000)], True),
+])
+def test_gradients_of_a_list_lie_apart(dcopy, spans, fine):
+    """Outputs overlap no gradient, no other output and not the workspace.  (Addresses only:
+    refused before anything is copied; what passes fails here for want of a GPU, if at all.)"""
+    if torch.cuda.is_available():
+        pytest.skip("made-up addresses")
+    base, size = 0x10000000, 100000
+    arr = (dcopy.DcopyGrad * len(spans))(*[(base + s, base + d, 100, 0, 0) for s, d in spans])
+    at = 20000 if (0, 20000) in spans else 200000
+    rc = dcopy.lib().dcopy_grad_list_build(ctypes.byref(dcopy.DcopyGradList()), arr, len(arr),
+                                           base + at, size, None)
+    message = dcopy.lib().dcopy_last_error_message()
+    assert (rc == dcopy.ERR_PARAM_INVALID and b"overlaps" in message) == (not fine), message
