@@ -269,6 +269,12 @@ int open_list(const DcopyGradList *list) {
   return check_device_span(list->workspace, list_bytes(list->first[kPairs]), "workspace");
 }
 
+// A number that a call on a list reads or writes lies apart from the list's workspace.
+int check_number(const DcopyGradList *list, const void *at, uint64_t bytes, const char *name) {
+  if (int rc = check_device_span(at, bytes, name)) return rc;
+  return check_disjoint(list->workspace, list_bytes(list->first[kPairs]), at, bytes, name);
+}
+
 // The chunks [begin, end) of a list.
 List part_of(const DcopyGradList *list, uint32_t begin, uint32_t end) {
   uint8_t *w = static_cast<uint8_t *>(list->workspace);
@@ -408,7 +414,7 @@ int dcopy_grad_list_build(DcopyGradList *list, const DcopyGrad *grads, uint32_t 
 int dcopy_grad_sum_squares(const DcopyGradList *list, double *total, dcopy_stream_t stream) {
   DCOPY_API_BEGIN
   if (int rc = open_list(list)) return rc;
-  if (int rc = check_device_span(total, sizeof(double), "total")) return rc;
+  if (int rc = check_number(list, total, sizeof(double), "total")) return rc;
   uint32_t parts = 0;
   if (int rc = run_sum(list, &parts, stream)) return rc;
   return launch(total_kernel, 1, dim3(kThreads), 0, stream, "total_kernel", part_of(list, 0, 0),
@@ -421,9 +427,11 @@ int dcopy_grad_clip(const DcopyGradList *list, const double *total, float max_no
   DCOPY_API_BEGIN
   if (int rc = check_bound(max_norm, eps, "grad_clip")) return rc;
   if (int rc = open_list(list)) return rc;
-  if (int rc = check_device_span(total, sizeof(double), "total")) return rc;
+  if (int rc = check_number(list, total, sizeof(double), "total")) return rc;
   if (norm)
-    if (int rc = check_device_span(norm, sizeof(float), "norm")) return rc;
+    if (int rc = check_number(list, norm, sizeof(float), "norm")) return rc;
+  if (int rc = check_disjoint(total, sizeof(double), norm, norm ? sizeof(float) : 0, "total, norm"))
+    return rc;
   return run_clip(list, 0, total, max_norm, eps, norm, stream);
   DCOPY_API_END
 }
@@ -434,7 +442,7 @@ int dcopy_clip_grad_norm(const DcopyGradList *list, float max_norm, float eps, f
   if (int rc = check_bound(max_norm, eps, "clip_grad_norm")) return rc;
   if (int rc = open_list(list)) return rc;
   if (norm)
-    if (int rc = check_device_span(norm, sizeof(float), "norm")) return rc;
+    if (int rc = check_number(list, norm, sizeof(float), "norm")) return rc;
   uint32_t parts = 0;
   if (int rc = run_sum(list, &parts, stream)) return rc;
   return run_clip(list, parts, nullptr, max_norm, eps, norm, stream);

@@ -394,8 +394,8 @@ int dcopy_embedding_lookup(const DcopyMatrix *out, const DcopyMatrix *table,
   if (out->cols > kMaxWidth)
     return set_error(DCOPY_ERR_UNSUPPORTED, "embedding_lookup: width %lld", (long long)out->cols);
   if (out->rows == 0 || out->cols == 0) return DCOPY_OK;
-  if (int rc = check_apart(out, table, "embedding_lookup")) return rc;
-  if (int rc = check_apart(out, ids, "embedding_lookup")) return rc;
+  if (int rc = check_apart(out, table, "embedding_lookup", "out", "table")) return rc;
+  if (int rc = check_apart(out, ids, "embedding_lookup", "out", "ids")) return rc;
   p.out = out->data;
   p.table = table->data;
   p.out_pitch = out->pitch;
@@ -462,10 +462,15 @@ int dcopy_embedding_grad(const DcopyMatrix *grad, const DcopyMatrix *dout, const
   if (src.n && workspace_bytes < need)
     return set_error(DCOPY_ERR_PARAM_INVALID, "embedding_grad: workspace of %llu bytes, %llu needed",
                      (unsigned long long)workspace_bytes, (unsigned long long)need);
-  if (src.n)
+  if (int rc = check_apart(grad, dout, "embedding_grad", "grad", "dout")) return rc;
+  if (int rc = check_apart(grad, ids, "embedding_grad", "grad", "ids")) return rc;
+  if (src.n) {
     if (int rc = check_device_span(workspace, need, "workspace")) return rc;
-  if (int rc = check_apart(grad, dout, "embedding_grad")) return rc;
-  if (int rc = check_apart(grad, ids, "embedding_grad")) return rc;
+    const DcopyMatrix space = flat(workspace, need, kU8);
+    if (int rc = check_apart(grad, &space, "embedding_grad", "grad", "workspace")) return rc;
+    if (int rc = check_apart(dout, &space, "embedding_grad", "dout", "workspace")) return rc;
+    if (int rc = check_apart(ids, &space, "embedding_grad", "ids", "workspace")) return rc;
+  }
   if (grad->rows == 0 || grad->cols == 0) return DCOPY_OK;
   Fill fill;
   if (!accumulate) {

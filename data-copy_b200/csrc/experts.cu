@@ -311,6 +311,16 @@ int check_route(const int32_t *dest, int64_t tokens, int64_t slots, const int32_
   return DCOPY_OK;
 }
 
+// What a call writes (`out`) lies apart from its routing.
+int check_off_route(const DcopyMatrix *out, const char *name, const int32_t *dest, uint64_t entries,
+                    const int32_t *source, uint64_t rows, const DcopyMatrix *weights,
+                    const char *what) {
+  const DcopyMatrix d = flat(dest, entries, kI32), s = flat(source, rows, kI32);
+  if (int rc = check_apart(out, &d, what, name, "dest")) return rc;
+  if (int rc = check_apart(out, &s, what, name, "source")) return rc;
+  return weights ? check_apart(out, weights, what, name, "weights") : (int)DCOPY_OK;
+}
+
 int check_width(const DcopyMatrix *a, const DcopyMatrix *b, const char *what) {
   if (a->type != b->type)
     return set_error(DCOPY_ERR_DATATYPE_INVALID, "%s: element types %d and %d differ", what,
@@ -400,6 +410,20 @@ int dcopy_expert_sort(int32_t *dest, int32_t *source, int64_t rows, int32_t *off
   if (int rc = check_device_span(offsets, ((uint64_t)experts + 1) * 4, "offsets")) return rc;
   if (need)
     if (int rc = check_device_span(workspace, need + 16, "workspace")) return rc;
+  // dest may be the ids themselves: an entry's id is read before its row is written, by
+  // the same block.
+  const DcopyMatrix out[] = {flat(dest, n, kI32), flat(source, (uint64_t)rows, kI32),
+                             flat(offsets, (uint64_t)experts + 1, kI32),
+                             flat(workspace, need ? need + 16 : 0, kU8)};
+  const char *const name[] = {"dest", "source", "offsets", "workspace"};
+  for (int i = 0; i < 4; ++i) {
+    for (int j = 0; j < i; ++j)
+      if (int rc = check_apart(&out[j], &out[i], "expert_sort", name[j], name[i])) return rc;
+    const bool in_place = i == 0 && expert_ids->data == dest && expert_ids->type == kI32 &&
+                          (expert_ids->rows <= 1 || expert_ids->pitch == expert_ids->cols);
+    if (!in_place)
+      if (int rc = check_apart(&out[i], expert_ids, "expert_sort", name[i], "expert_ids")) return rc;
+  }
   KeySource src{};
   src.ids = expert_ids->data;
   src.pitch = expert_ids->pitch;
@@ -424,7 +448,10 @@ int dcopy_expert_dispatch(const DcopyMatrix *out, const DcopyMatrix *x, const in
   if (int rc = check_width(out, x, "expert_dispatch")) return rc;
   if (int rc = check_route(dest, x->rows, slots, source, out->rows, weights, "expert_dispatch"))
     return rc;
-  if (int rc = check_apart(out, x, "expert_dispatch")) return rc;
+  if (int rc = check_apart(out, x, "expert_dispatch", "out", "x")) return rc;
+  if (int rc = check_off_route(out, "out", dest, (uint64_t)x->rows * slots, source, out->rows,
+                               weights, "expert_dispatch"))
+    return rc;
   if (out->rows == 0 || out->cols == 0) return DCOPY_OK;
   Route p{};
   p.out = out->data;
@@ -479,7 +506,10 @@ int dcopy_expert_combine(const DcopyMatrix *out, const DcopyMatrix *y, const int
   if (int rc = check_matrix(y, "y", is_float(y->type))) return rc;
   if (int rc = check_width(out, y, "expert_combine")) return rc;
   if (int rc = check_route(dest, out->rows, slots, nullptr, 0, weights, "expert_combine")) return rc;
-  if (int rc = check_apart(out, y, "expert_combine")) return rc;
+  if (int rc = check_apart(out, y, "expert_combine", "out", "y")) return rc;
+  if (int rc = check_off_route(out, "out", dest, (uint64_t)out->rows * slots, nullptr, 0, weights,
+                               "expert_combine"))
+    return rc;
   if (out->rows == 0 || out->cols == 0) return DCOPY_OK;
   Route p{};
   p.out = out->data;
@@ -532,8 +562,19 @@ int dcopy_expert_combine_grad(const DcopyMatrix *dy, const DcopyMatrix *dweights
                      "expert_combine_grad: dy has %lld rows for %lld of y, dweights is %lld x %lld",
                      (long long)dy->rows, (long long)y->rows, (long long)dweights->rows,
                      (long long)dweights->cols);
-  if (int rc = check_apart(dy, y, "expert_combine_grad")) return rc;
-  if (int rc = check_apart(dy, dout, "expert_combine_grad")) return rc;
+  // dweights may be the weights themselves: an entry's weight is read before its gradient
+  // is written, by the same warp or behind a barrier.
+  const char *what = "expert_combine_grad";
+  const uint64_t all = (uint64_t)dout->rows * slots;
+  const DcopyMatrix *other = same_rows(dweights, weights) ? nullptr : weights;
+  if (int rc = check_apart(dy, y, what, "dy", "y")) return rc;
+  if (int rc = check_apart(dy, dout, what, "dy", "dout")) return rc;
+  if (int rc = check_apart(dy, dweights, what, "dy", "dweights")) return rc;
+  if (int rc = check_apart(dweights, y, what, "dweights", "y")) return rc;
+  if (int rc = check_apart(dweights, dout, what, "dweights", "dout")) return rc;
+  if (int rc = check_off_route(dy, "dy", dest, all, source, dy->rows, weights, what)) return rc;
+  if (int rc = check_off_route(dweights, "dweights", dest, all, source, dy->rows, other, what))
+    return rc;
   Route p{};
   p.out = dy->data;
   p.in = y->data;

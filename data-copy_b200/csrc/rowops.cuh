@@ -63,8 +63,35 @@ inline uint64_t matrix_span(const DcopyMatrix *m) {
   return ((uint64_t)(m->rows - 1) * (m->rows > 1 ? m->pitch : 0) + m->cols) * elem_size(m->type);
 }
 
-inline int check_apart(const DcopyMatrix *a, const DcopyMatrix *b, const char *what) {
-  return check_disjoint(a->data, matrix_span(a), b->data, matrix_span(b), what);
+// Whether no byte belongs to rows of both.  Rows of one pitch may interleave, as column
+// slices of one buffer do.
+inline bool apart(const DcopyMatrix *a, const DcopyMatrix *b) {
+  const uintptr_t pa = (uintptr_t)a->data, pb = (uintptr_t)b->data;
+  const uint64_t na = matrix_span(a), nb = matrix_span(b);
+  if (!na || !nb || pa >= pb + nb || pb >= pa + na) return true;
+  const uint64_t ea = elem_size(a->type), eb = elem_size(b->type);
+  const uint64_t step_a = a->rows > 1 ? a->pitch * ea : 0, step_b = b->rows > 1 ? b->pitch * eb : 0;
+  const uint64_t step = step_a ? step_a : step_b;
+  if (!step || (step_b && step_b != step)) return false;
+  const uint64_t at = pb >= pa ? (pb - pa) % step : (step - (pa - pb) % step) % step;
+  return at >= a->cols * ea && at + b->cols * eb <= step;
+}
+
+inline int check_apart(const DcopyMatrix *a, const DcopyMatrix *b, const char *what,
+                       const char *name_a, const char *name_b) {
+  if (apart(a, b)) return DCOPY_OK;
+  return set_error(DCOPY_ERR_PARAM_INVALID, "%s: %s and %s overlap", what, name_a, name_b);
+}
+
+// Whether b is a itself.
+inline bool same_rows(const DcopyMatrix *a, const DcopyMatrix *b) {
+  return a->data == b->data && a->type == b->type && a->rows == b->rows && a->cols == b->cols &&
+         (a->rows <= 1 || a->pitch == b->pitch);
+}
+
+// An array as a matrix of one row; NULL is empty.
+inline DcopyMatrix flat(const void *data, uint64_t count, int32_t type) {
+  return DcopyMatrix{const_cast<void *>(data), 1, data ? (int64_t)count : 0, 0, type, 0};
 }
 
 // Largest V in {8, 4, 2, 1} of at most 16 bytes for which a row of the matrix is whole

@@ -510,7 +510,9 @@ int dcopy_memcpy_async_batch(const DcopyMemcpyInfo *infos, uint32_t count, int32
  * reference has no counterpart.  Elements are FLOAT (0), FLOAT16 (1) or BF16 (27);
  * sums are held in fp32 and rounded once, to nearest even.  Every result is the
  * same on every run: no sum depends on the order in which blocks execute.  Widths
- * beyond 2^23 are UNSUPPORTED, rows and ids beyond 2^31 - 1 SHAPE_INVALID. */
+ * beyond 2^23 are UNSUPPORTED, rows and ids beyond 2^31 - 1 SHAPE_INVALID.  What a call
+ * writes, its workspace included, overlaps none of its other arguments unless said so
+ * (rows of one pitch may interleave, as column slices of one buffer do). */
 
 /* rows x cols elements of a GE DataType, rows `pitch` elements apart (at least
  * cols; not looked at when rows <= 1).  data is aligned to the element. */
@@ -524,7 +526,7 @@ typedef struct DcopyMatrix {
 /* out[i,:] = round(scale * table[id_i - first_id, :]), zero where id_i - first_id
  * lies outside the table (a padding id, or another rank's part of a vocabulary that
  * is split by rows).  ids: INT32 (3) or INT64 (9), read row by row; out has a row
- * for each id.  out and table may differ in type.  out overlaps neither input. */
+ * for each id.  out and table may differ in type. */
 int dcopy_embedding_lookup(const DcopyMatrix *out, const DcopyMatrix *table,
                            const DcopyMatrix *ids, int64_t first_id, float scale,
                            dcopy_stream_t stream);
@@ -545,7 +547,8 @@ int dcopy_embedding_grad(const DcopyMatrix *grad, const DcopyMatrix *dout, const
  * no expert; the rows of expert x are [offsets[x], offsets[x+1]), its entries first
  * and in entry order, offsets[x+1] - offsets[x] rounded up to a multiple of `align`.
  * source[row] is the entry of a row, -1 where a row holds none.  rows, the length of
- * source, is at least dcopy_expert_rows; experts is at most 1023. */
+ * source, is at least dcopy_expert_rows; experts is at most 1023.  dest may be
+ * expert_ids itself (INT32, dense). */
 int dcopy_expert_rows(int64_t entries, int32_t experts, int32_t align, int64_t *rows);
 int dcopy_expert_sort_workspace(int64_t entries, int32_t experts, uint64_t *bytes);
 int dcopy_expert_sort(int32_t *dest, int32_t *source, int64_t rows, int32_t *offsets,
@@ -567,7 +570,8 @@ int dcopy_expert_combine(const DcopyMatrix *out, const DcopyMatrix *y, const int
                          int64_t slots, const DcopyMatrix *weights, dcopy_stream_t stream);
 /* The gradient of dcopy_expert_combine: dy[dest[i,j],:] = round(weights[i,j] * dout[i,:])
  * and dweights[i,j] = sum of dout[i,:] * y[dest[i,j],:] (FLOAT; 0 for skipped entries).
- * source as in dcopy_expert_dispatch, for the rows of dy. */
+ * source as in dcopy_expert_dispatch, for the rows of dy.  dweights may be weights
+ * itself. */
 int dcopy_expert_combine_grad(const DcopyMatrix *dy, const DcopyMatrix *dweights,
                               const DcopyMatrix *dout, const DcopyMatrix *y, const int32_t *dest,
                               int64_t slots, const int32_t *source, const DcopyMatrix *weights,

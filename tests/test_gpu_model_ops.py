@@ -621,3 +621,34 @@ def test_refusals_on_the_gpu(torch_cuda, dcopy):
     base = torch.ones(100, device="cuda")
     refused(dcopy.ERR_PARAM_INVALID, dcopy.GradList, [base[:50]], [base[10:60]])
     refused(dcopy.ERR_PARAM_INVALID, dcopy.clip_grad_norm, dcopy.GradList([base]), float("nan"))
+
+
+@pytest.mark.parametrize("n", [100, 5000])
+def test_sort_in_place(torch_cuda, dcopy, n):
+    """The routing written over the choices that it is made of."""
+    case = (n, 3, 17, 4, 0.1)
+    ids = routing(gen(n), case, torch.int32)
+    d, s, o = sort_exact(ids, 17, 4, dcopy.expert_rows(3 * n, 17, 4))
+    source = torch.empty(len(s), dtype=torch.int32, device="cuda")
+    offsets = torch.empty(18, dtype=torch.int32, device="cuda")
+    dcopy.expert_sort(ids, source, offsets, ids, align=4)
+    assert np.array_equal(ids.cpu().numpy(), d) and np.array_equal(source.cpu().numpy(), s)
+    assert np.array_equal(offsets.cpu().numpy(), o)
+
+
+@pytest.mark.parametrize("n,width", [(2000, 24), (2000, 4096), (40, 4096)])
+def test_weight_gradients_in_place_and_beside(torch_cuda, dcopy, n, width):
+    """The weights' gradients written over the weights, and into columns beside them."""
+    case = (n, 4, 16, 1, 0.1)
+    g = gen(width)
+    dest, source, _ = sorted_route(dcopy, routing(g, case), case)
+    dout, y = randn(g, (n, width), BF16), randn(g, (source.numel(), width), BF16)
+    both = randn(g, (n, 8), F32)
+    w = both[:, :4].clone()
+    dy, dw = torch.empty_like(y), torch.empty_like(w)
+    dcopy.expert_combine_grad(dy, dw, dout, y, dest, w, source)
+    got = torch.empty_like(dy)
+    dcopy.expert_combine_grad(got, both[:, 4:], dout, y, dest, both[:, :4], source)
+    assert torch.equal(got, dy) and torch.equal(both[:, 4:], dw) and torch.equal(both[:, :4], w)
+    dcopy.expert_combine_grad(got, w, dout, y, dest, w, source)
+    assert torch.equal(got, dy) and torch.equal(w, dw)

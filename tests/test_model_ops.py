@@ -143,3 +143,128 @@ def test_gradients_of_a_list_lie_apart(dcopy, spans, fine):
                                            base + at, size, None)
     message = dcopy.lib().dcopy_last_error_message()
     assert (rc == dcopy.ERR_PARAM_INVALID and b"overlaps" in message) == (not fine), message
+
+
+BASE = 0x20000000
+PLACES = {  # argument -> (offset, rows, cols, pitch, type code); 64 tokens x 4 slots, 256 rows, 8 experts
+    "lookup": dict(out=(0, 64, 32, 32, 0), table=(1 << 20, 100, 32, 32, 0), ids=(2 << 20, 64, 1, 1, 9)),
+    "grad": dict(grad=(0, 100, 32, 32, 0), dout=(1 << 20, 64, 32, 32, 0), ids=(2 << 20, 64, 1, 1, 9),
+                 workspace=(3 << 20, 1, 0, 0, 4)),  # as many bytes as are needed, here and below
+    "sort": dict(dest=(0, 1, 6400, 0, 3), source=(1 << 20, 1, 6400, 0, 3), offsets=(2 << 20, 1, 9, 0, 3),
+                 expert_ids=(3 << 20, 1600, 4, 4, 3), workspace=(4 << 20, 1, 0, 0, 4)),
+    "dispatch": dict(out=(0, 256, 32, 32, 0), x=(1 << 20, 64, 32, 32, 0), dest=(2 << 20, 1, 256, 0, 3),
+                     source=(3 << 20, 1, 256, 0, 3), weights=(4 << 20, 64, 4, 4, 0)),
+    "combine": dict(out=(0, 64, 32, 32, 0), y=(1 << 20, 256, 32, 32, 0), dest=(2 << 20, 1, 256, 0, 3),
+                    weights=(4 << 20, 64, 4, 4, 0)),
+    "combine_grad": dict(dy=(0, 256, 32, 32, 0), dweights=(1 << 20, 64, 4, 4, 0),
+                         dout=(2 << 20, 64, 32, 32, 0), y=(3 << 20, 256, 32, 32, 0),
+                         dest=(4 << 20, 1, 256, 0, 3), source=(5 << 20, 1, 256, 0, 3),
+                         weights=(6 << 20, 64, 4, 4, 0)),
+}
+WRITTEN = {"lookup": ["out"], "grad": ["grad", "workspace"], "sort": ["dest", "source", "offsets", "workspace"],
+           "dispatch": ["out"], "combine": ["out"], "combine_grad": ["dy", "dweights"]}
+
+
+def places_of(dcopy, op):
+    need = {"grad": lambda: dcopy.embedding_grad_workspace(64, 100, 32),
+            "sort": lambda: dcopy.expert_sort_workspace(6400, 8)}
+    return {k: (at, r, need[op]() if k == "workspace" else c, p, t)
+            for k, (at, r, c, p, t) in PLACES[op].items()}
+
+
+def call_at(dcopy, op, places):
+    """Status and message of a call on made-up addresses."""
+    if torch.cuda.is_available():
+        pytest.skip("made-up addresses")
+    m = {k: dcopy.DcopyMatrix(BASE + at, r, c, p, t, 0) for k, (at, r, c, p, t) in places.items()}
+    ref = {k: ctypes.byref(v) for k, v in m.items()}
+    raw = {k: v.data for k, v in m.items()}
+    lib = dcopy.lib()
+    rc = {
+        "lookup": lambda: lib.dcopy_embedding_lookup(ref["out"], ref["table"], ref["ids"], 0, 1.0, None),
+        "grad": lambda: lib.dcopy_embedding_grad(ref["grad"], ref["dout"], ref["ids"], 0, 1.0, 0,
+                                                 raw["workspace"], m["workspace"].cols, None),
+        "sort": lambda: lib.dcopy_expert_sort(raw["dest"], raw["source"], m["source"].cols, raw["offsets"],
+                                              ref["expert_ids"], 8, 1, raw["workspace"],
+                                              m["workspace"].cols, None),
+        "dispatch": lambda: lib.dcopy_expert_dispatch(ref["out"], ref["x"], raw["dest"], 4, raw["source"],
+                                                      ref["weights"], None),
+        "combine": lambda: lib.dcopy_expert_combine(ref["out"], ref["y"], raw["dest"], 4, ref["weights"], None),
+        "combine_grad": lambda: lib.dcopy_expert_combine_grad(
+            ref["dy"], ref["dweights"], ref["dout"], ref["y"], raw["dest"], 4, raw["source"],
+            ref["weights"], None),
+    }[op]()
+    return rc, lib.dcopy_last_error_message()
+
+
+def overlaps(dcopy, op, places):
+    rc, message = call_at(dcopy, op, places)
+    assert rc != dcopy.OK  # no GPU
+    return rc == dcopy.ERR_PARAM_INVALID and b"overlap" in message
+
+
+@pytest.mark.parametrize("op,written,other", [(op, w, o) for op in PLACES for w in WRITTEN[op]
+                                              for o in PLACES[op] if o != w])
+def test_what_is_written_lies_apart(dcopy, op, written, other):
+    """Whatever a call writes overlaps no other argument, at its first byte or its last."""
+    places = places_of(dcopy, op)
+    assert not overlaps(dcopy, op, places)
+    start, rows, cols, pitch, code = places[other]
+    wide = {0: 4, 3: 4, 4: 1, 9: 8}
+    first, w_rows, w_cols, w_pitch, w_code = places[written]
+    last = first + ((w_rows - 1) * w_pitch + w_cols - 1) * wide[w_code]
+    for at in (first + 8, last // 8 * 8):
+        assert overlaps(dcopy, op, {**places, other: (at, rows, cols, pitch, code)}), at
+    end = (last + wide[w_code] + 15) // 16 * 16
+    # Behind its last byte, well before the next argument.
+    assert not overlaps(dcopy, op, {**places, other: (end, rows, cols, pitch, code)})
+
+
+def test_what_may_be_in_place(dcopy):
+    """The routing written over the choices it is made of, and weights' gradients over the
+    weights; neither at another place of the same memory nor in another type."""
+    sort, back = places_of(dcopy, "sort"), places_of(dcopy, "combine_grad")
+    at = sort["dest"][0]
+    assert not overlaps(dcopy, "sort", {**sort, "expert_ids": (at, 1600, 4, 4, 3)})
+    assert overlaps(dcopy, "sort", {**sort, "expert_ids": (at, 1600, 4, 5, 3)})
+    assert overlaps(dcopy, "sort", {**sort, "expert_ids": (at, 1600, 4, 4, 9)})
+    assert overlaps(dcopy, "sort", {**sort, "expert_ids": (at + 4, 1600, 4, 4, 3)})
+    at = back["dweights"][0]
+    assert not overlaps(dcopy, "combine_grad", {**back, "weights": (at, 64, 4, 4, 0)})
+    assert overlaps(dcopy, "combine_grad", {**back, "weights": (at, 64, 4, 5, 0)})
+    assert overlaps(dcopy, "combine_grad", {**back, "weights": (at + 4, 64, 4, 4, 0)})
+
+
+def test_columns_of_one_buffer_lie_apart(dcopy):
+    """Rows of one pitch that interleave share no byte."""
+    back = places_of(dcopy, "combine_grad")
+    dw, w = (1 << 20, 64, 4, 8, 0), ((1 << 20) + 16, 64, 4, 8, 0)
+    assert not overlaps(dcopy, "combine_grad", {**back, "dweights": dw, "weights": w})
+    assert not overlaps(dcopy, "combine_grad", {**back, "dweights": w, "weights": dw})
+    for at in (12, 20, 32 + 12):  # a column shared, behind a slice or before the next row's
+        moved = ((1 << 20) + at, 64, 4, 8, 0)
+        assert overlaps(dcopy, "combine_grad", {**back, "dweights": dw, "weights": moved})
+        assert overlaps(dcopy, "combine_grad", {**back, "dweights": moved, "weights": dw})
+    assert overlaps(dcopy, "combine_grad", {**back, "dweights": dw, "weights": (*w[:3], 12, 0)})
+    look = places_of(dcopy, "lookup")
+    assert not overlaps(dcopy, "lookup", {**look, "out": (0, 64, 32, 64, 0), "table": (128, 100, 32, 64, 0)})
+    assert overlaps(dcopy, "lookup", {**look, "out": (0, 64, 32, 64, 0), "table": (124, 100, 32, 64, 0)})
+
+
+def test_numbers_of_a_clipping_call_lie_apart(dcopy):
+    """The sum and the norm lie outside the list's workspace, and the norm outside the sum."""
+    if torch.cuda.is_available():
+        pytest.skip("made-up addresses")
+    lib, built = dcopy.lib(), dcopy.DcopyGradList()
+    built.workspace = BASE
+
+    def refused(rc):
+        return rc == dcopy.ERR_PARAM_INVALID and b"overlap" in lib.dcopy_last_error_message()
+
+    ref, far = ctypes.byref(built), BASE + (1 << 20)
+    assert refused(lib.dcopy_grad_sum_squares(ref, BASE + 64, None))
+    assert refused(lib.dcopy_grad_clip(ref, BASE + 64, 1.0, 0.0, None, None))
+    assert refused(lib.dcopy_grad_clip(ref, far, 1.0, 0.0, BASE + 64, None))
+    assert refused(lib.dcopy_grad_clip(ref, far, 1.0, 0.0, far + 4, None))
+    assert refused(lib.dcopy_clip_grad_norm(ref, 1.0, 0.0, BASE, None))
+    assert not refused(lib.dcopy_grad_clip(ref, far, 1.0, 0.0, far + 8, None))
