@@ -91,14 +91,14 @@ DcopyMatrix layout(const at::Tensor &t, const char *name) {
     m.pitch = stride[d - 2];
     m.rows = 1;
     for (int64_t k = d - 2; k >= 0; --k) {
-      if (shape[k] > 1) {
+      if (shape[k] > 1 && t.numel()) {  // without elements strides mean nothing
         if (m.rows == 1) m.pitch = stride[k];
         else if (stride[k] != m.rows * m.pitch) value_error(name, "rows do not lie at one pitch");
       }
       m.rows *= shape[k];
     }
   }
-  if (unit != 1 && m.cols > 1) value_error(name, "the last dimension must be dense");
+  if (unit != 1 && m.cols > 1 && t.numel()) value_error(name, "the last dimension must be dense");
   m.data = const_cast<void *>(t.const_data_ptr());
   m.type = type_code(t.scalar_type());
   return m;

@@ -652,3 +652,27 @@ def test_weight_gradients_in_place_and_beside(torch_cuda, dcopy, n, width):
     assert torch.equal(got, dy) and torch.equal(both[:, 4:], dw) and torch.equal(both[:, :4], w)
     dcopy.expert_combine_grad(got, w, dout, y, dest, w, source)
     assert torch.equal(got, dy) and torch.equal(w, dw)
+
+
+@pytest.mark.parametrize("shape", [(4, 0), (0, 4), (0,), (2, 3, 0)])
+def test_empty_batches_of_any_shape(torch_cuda, dcopy, shape):
+    """Batches without a token, with the zero in any place, as a training loop's last may be."""
+    ids = torch.zeros(shape, dtype=torch.int64, device="cuda")
+    table, x = torch.randn(9, 16, device="cuda"), torch.empty(*shape, 16, device="cuda")
+    dcopy.embedding_lookup(x, table, ids, scale=2.0)
+    grad = torch.full_like(table, 3.0)
+    dcopy.embedding_grad(grad, x, ids)
+    assert bool((grad == 0).all())
+    chosen, w = ids[..., None].expand(*shape, 2).contiguous(), torch.empty(*shape, 2, device="cuda")
+    dest = torch.empty(*shape, 2, dtype=torch.int32, device="cuda")
+    source = torch.full((5,), 7, dtype=torch.int32, device="cuda")
+    offsets = torch.full((4,), 7, dtype=torch.int32, device="cuda")
+    dcopy.expert_sort(dest, source, offsets, chosen, align=4)
+    assert offsets.tolist() == [0] * 4 and source.tolist() == [-1] * 5
+    rows, dw = torch.full((5, 16), 3.0, device="cuda"), torch.empty_like(w)
+    dcopy.expert_dispatch(rows, x, dest, source)
+    assert bool((rows == 0).all())
+    dcopy.expert_combine(x, rows, dest, w)
+    dy = torch.full_like(rows, 3.0)
+    dcopy.expert_combine_grad(dy, dw, x, rows, dest, w, source)
+    assert bool((dy == 0).all())

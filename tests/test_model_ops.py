@@ -268,3 +268,22 @@ def test_numbers_of_a_clipping_call_lie_apart(dcopy):
     assert refused(lib.dcopy_grad_clip(ref, far, 1.0, 0.0, far + 4, None))
     assert refused(lib.dcopy_clip_grad_norm(ref, 1.0, 0.0, BASE, None))
     assert not refused(lib.dcopy_grad_clip(ref, far, 1.0, 0.0, far + 8, None))
+
+
+def test_layout_of_an_empty_tensor(dcopy):
+    """An empty batch has rows, columns and no pitch to disagree about, wherever its zero is."""
+    from dcopy import model_ops
+
+    def read(*shape):
+        rows, cols, _, code = model_ops._calls.layout(torch.zeros(*shape))
+        assert code == 0
+        return rows, cols
+
+    assert read(4, 0, 8) == (0, 8) and read(0, 4, 8) == (0, 8) and read(3, 4, 0, 8) == (0, 8)
+    assert read(2, 0, 5, 8) == (0, 8) and read(4, 5, 0) == (20, 0) and read(0) == (1, 0)
+    rows, cols, _, _ = model_ops._calls.layout(torch.zeros(6, 0, 16).transpose(0, 1))
+    assert (rows, cols) == (0, 16)
+    rows, cols, _, _ = model_ops._calls.layout(torch.zeros(0, 6).t())
+    assert (rows, cols) == (6, 0)
+    rows, cols, _, _ = model_ops._calls.layout(torch.zeros(6, 0).t())
+    assert (rows, cols) == (0, 6)
