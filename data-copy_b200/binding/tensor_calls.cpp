@@ -274,18 +274,20 @@ PyObject *expert_sort(PyObject *, PyObject *const *a, Py_ssize_t n) {
   });
 }
 
-// dest and source of a routing of `tokens` tokens into `rows` rows.
+// dest and source of a routing of `tokens` tokens into `rows` rows.  A flat dest has as
+// many slots as divide it over the tokens, without tokens those of the weights.
 struct Routing {
   const int32_t *dest, *source;
   int64_t slots;
 };
-Routing routing(Call &c, PyObject *dest, PyObject *source, int64_t tokens, int64_t rows) {
+Routing routing(Call &c, PyObject *dest, PyObject *source, int64_t tokens, int64_t rows,
+                const DcopyMatrix &weights) {
   Routing r{};
   int64_t n = 0, held = rows;
   r.dest = (const int32_t *)c.vector(dest, "dest", at::kInt, &n);
   r.source = (const int32_t *)c.vector(source, "source", at::kInt, &held);
   if (dest != Py_None && unpack(dest, "dest").dim() > 1) r.slots = unpack(dest, "dest").size(-1);
-  else r.slots = tokens ? n / tokens : 0;
+  else r.slots = tokens ? n / tokens : weights.cols;
   if (r.slots * tokens != n)
     dcopy_error(DCOPY_ERR_SHAPE_INVALID, "dest has " + std::to_string(n) + " values for " +
                 std::to_string(tokens) + " tokens", c.func());
@@ -298,10 +300,10 @@ Routing routing(Call &c, PyObject *dest, PyObject *source, int64_t tokens, int64
 PyObject *expert_dispatch(PyObject *, PyObject *const *a, Py_ssize_t n) {
   return run("dcopy_expert_dispatch", a, n, 6, [&](Call &c) {
     const DcopyMatrix out = c.matrix(a[0], "out"), x = c.matrix(a[1], "x");
-    const Routing r = routing(c, a[2], a[3], x.rows, out.rows);
     DcopyMatrix weights{};
     const bool weighted = a[4] != Py_None;
     if (weighted) weights = c.matrix(a[4], "weights");
+    const Routing r = routing(c, a[2], a[3], x.rows, out.rows, weights);
     dcopy_stream_t s = c.stream();
     c.check(unlocked([&] {
       return lib.dcopy_expert_dispatch(&out, &x, r.dest, r.slots, r.source,
@@ -313,10 +315,10 @@ PyObject *expert_dispatch(PyObject *, PyObject *const *a, Py_ssize_t n) {
 PyObject *expert_combine(PyObject *, PyObject *const *a, Py_ssize_t n) {
   return run("dcopy_expert_combine", a, n, 5, [&](Call &c) {
     const DcopyMatrix out = c.matrix(a[0], "out"), y = c.matrix(a[1], "y");
-    const Routing r = routing(c, a[2], Py_None, out.rows, y.rows);
     DcopyMatrix weights{};
     const bool weighted = a[3] != Py_None;
     if (weighted) weights = c.matrix(a[3], "weights");
+    const Routing r = routing(c, a[2], Py_None, out.rows, y.rows, weights);
     dcopy_stream_t s = c.stream();
     c.check(unlocked([&] {
       return lib.dcopy_expert_combine(&out, &y, r.dest, r.slots, weighted ? &weights : nullptr, s);
@@ -329,7 +331,7 @@ PyObject *expert_combine_grad(PyObject *, PyObject *const *a, Py_ssize_t n) {
     const DcopyMatrix dy = c.matrix(a[0], "dy"), dw = c.matrix(a[1], "dweights"),
                       dout = c.matrix(a[2], "dout"), y = c.matrix(a[3], "y"),
                       weights = c.matrix(a[5], "weights");
-    const Routing r = routing(c, a[4], a[6], dout.rows, dy.rows);
+    const Routing r = routing(c, a[4], a[6], dout.rows, dy.rows, weights);
     dcopy_stream_t s = c.stream();
     c.check(unlocked([&] {
       return lib.dcopy_expert_combine_grad(&dy, &dw, &dout, &y, r.dest, r.slots, r.source, &weights,

@@ -676,3 +676,25 @@ def test_empty_batches_of_any_shape(torch_cuda, dcopy, shape):
     dy = torch.full_like(rows, 3.0)
     dcopy.expert_combine_grad(dy, dw, x, rows, dest, w, source)
     assert bool((dy == 0).all())
+
+
+@pytest.mark.parametrize("n", [0, 1, 50])
+def test_flat_routing_of_one_slot(torch_cuda, dcopy, n):
+    """A router that picks one expert a token, its choices a vector; no tokens too."""
+    g = gen(n)
+    ids = torch.randint(0, 3, (n,), generator=g, device="cuda")
+    dest, offsets = torch.empty(n, dtype=torch.int32, device="cuda"), torch.empty(4, dtype=torch.int32, device="cuda")
+    source = torch.empty(dcopy.expert_rows(n, 3, 4), dtype=torch.int32, device="cuda")
+    dcopy.expert_sort(dest, source, offsets, ids, align=4)
+    x, w = randn(g, (n, 8), F32), randn(g, (n, 1), F32)
+    rows, out, dw = torch.empty(source.numel(), 8, device="cuda"), torch.empty_like(x), torch.empty_like(w)
+    dcopy.expert_dispatch(rows, x, dest, source, w)
+    assert torch.equal(rows[dest.long()], x * w)
+    dcopy.expert_dispatch(rows, x, dest, source)
+    dcopy.expert_combine(out, rows, dest, w)
+    assert torch.equal(out, x * w)
+    dy = torch.empty_like(rows)
+    dcopy.expert_combine_grad(dy, dw, x, rows, dest, w, source)
+    assert torch.equal(dy[dest.long()], x * w)
+    exact = (x.double() ** 2).sum(1, keepdim=True)
+    close(dw, exact, 16, exact)
