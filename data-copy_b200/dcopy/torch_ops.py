@@ -259,7 +259,8 @@ def _dense(t: torch.Tensor) -> torch.Tensor:
 def embedding(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0,
               first_id: int = 0) -> torch.Tensor:
     out = table.new_empty(list(ids.shape) + [table.shape[1]])
-    dcopy.embedding_lookup(out.view(-1, table.shape[1]), table, ids.contiguous(), scale, first_id)
+    dcopy.embedding_lookup(out.view(ids.numel(), table.shape[1]), table, ids.contiguous(), scale,
+                           first_id)
     return out
 
 
@@ -273,7 +274,7 @@ def embedding_backward(dout: torch.Tensor, ids: torch.Tensor, vocab: int, scale:
                        first_id: int = 0) -> torch.Tensor:
     width = dout.shape[-1]
     grad = dout.new_empty(vocab, width)
-    dcopy.embedding_grad(grad, _dense(dout).view(-1, width), ids.contiguous(), scale, first_id)
+    dcopy.embedding_grad(grad, _dense(dout).view(ids.numel(), width), ids.contiguous(), scale, first_id)
     return grad
 
 

@@ -106,3 +106,18 @@ def test_training_example(torch_cuda):
     assert abs(a[0][0] - b[0][0]) <= 1e-4 * b[0][0] and abs(a[0][1] - b[0][1]) <= 1e-4 * b[0][1]
     assert all(abs(x[0] - y[0]) <= 1e-2 * y[0] for x, y in zip(a, b))
     assert a[-1][0] < a[0][0]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(4, 3), (0,), (4, 0)])
+@pytest.mark.parametrize("width", [0, 8])
+def test_embedding_without_elements(ops, torch_cuda, shape, width):
+    """Tables without columns and batches without tokens, there and back."""
+    ids = torch.zeros(shape, dtype=torch.int64, device="cuda")
+    table = torch.randn(5, width, device="cuda", requires_grad=True)
+    out = ops.embedding(table, ids, 2.0)
+    assert torch.equal(out, table[ids] * 2.0)
+    grad, = torch.autograd.grad(out.sum(), table)
+    want = torch.zeros(5, width, device="cuda")
+    want[:1] = 2.0 * ids.numel()
+    assert torch.equal(grad, want)
