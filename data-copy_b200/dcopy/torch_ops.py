@@ -308,11 +308,18 @@ def expert_sort(expert_ids: torch.Tensor, experts: int,
     return dest, source, offsets
 
 
+def _expert_rows(entries, experts, align):
+    """dcopy.expert_rows; where a number is symbolic, its formula, so that it stays so."""
+    if all(isinstance(n, int) for n in (entries, experts, align)):
+        return dcopy.expert_rows(entries, experts, align)
+    return entries + torch.sym_min(experts, entries) * (align - 1)
+
+
 @expert_sort.register_fake
 def _expert_sort_fake(expert_ids, experts, align=1):
     whole = dict(dtype=torch.int32)
     return (expert_ids.new_empty(expert_ids.shape, **whole),
-            expert_ids.new_empty(dcopy.expert_rows(expert_ids.numel(), experts, align), **whole),
+            expert_ids.new_empty(_expert_rows(expert_ids.numel(), experts, align), **whole),
             expert_ids.new_empty(experts + 1, **whole))
 
 

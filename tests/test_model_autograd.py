@@ -48,3 +48,41 @@ def test_hooks_see_what_is_kept(ops, weighted, count):
         assert len(seen) == count
         for out, _ in outs.values():
             out.sum().backward()
+
+
+@pytest.mark.parametrize("align", [1, 16])
+def test_token_counts_stay_symbolic(dcopy, ops, align):
+    """Traced with dynamic shapes, the rows of a routing follow the token count: nothing turns
+    it into the number of the example."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    def step(chosen, x):
+        dest, source, offsets = ops.expert_sort(chosen, 4, align)
+        return ops.expert_combine(ops.expert_dispatch(x, dest, source), dest, source), source
+
+    traced = make_fx(step, tracing_mode="symbolic")(torch.zeros(10, 2, dtype=torch.int64),
+                                                    torch.zeros(10, 8))
+    rows = next(n for n in traced.graph.nodes if "expert_dispatch" in str(n.target)).meta["val"].shape[0]
+    assert isinstance(rows, torch.SymInt)
+    expr = rows.node.expr
+    assert len(expr.free_symbols) == 2  # tokens and slots
+    for tokens, slots in ((5, 3), (1, 1), (300, 2)):
+        sizes = dict(zip(expr.free_symbols, (tokens, slots)))
+        assert int(expr.subs(sizes)) == dcopy.expert_rows(tokens * slots, 4, align)
+
+
+@pytest.mark.gpu
+def test_opcheck_with_dynamic_shapes(ops, torch_cuda):
+    """The operators traced for all sizes give what they give when called."""
+    from torch.library import opcheck
+    chosen = torch.randint(-1, 4, (30, 3), device="cuda")
+    dest, source, _ = ops.expert_sort(chosen, 4, 8)
+    x = torch.randn(30, 20, device="cuda", requires_grad=True)
+    w = torch.randn(30, 3, device="cuda", requires_grad=True)
+    y = torch.randn(source.numel(), 20, device="cuda", requires_grad=True)
+    table = torch.randn(9, 8, device="cuda", requires_grad=True)
+    for op, args in ((ops.embedding, (table, chosen)), (ops.expert_sort, (chosen, 4, 8)),
+                     (ops.expert_dispatch, (x, dest, source)), (ops.expert_combine, (y, dest, source, w)),
+                     (ops.expert_combine, (y, dest, source))):
+        opcheck(op, args, test_utils=("test_schema", "test_autograd_registration", "test_faketensor",
+                                      "test_aot_dispatch_dynamic"))
