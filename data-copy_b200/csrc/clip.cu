@@ -271,7 +271,7 @@ int open_list(const DcopyGradList *list) {
 
 // A number that a call on a list reads or writes lies apart from the list's workspace.
 int check_number(const DcopyGradList *list, const void *at, uint64_t bytes, const char *name) {
-  if (int rc = check_device_span(at, bytes, name)) return rc;
+  if (int rc = check_array(at, 1, bytes, name)) return rc;
   return check_disjoint(list->workspace, list_bytes(list->first[kPairs]), at, bytes, name);
 }
 

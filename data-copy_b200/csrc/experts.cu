@@ -298,9 +298,9 @@ int check_route(const int32_t *dest, int64_t tokens, int64_t slots, const int32_
     return set_error(DCOPY_ERR_SHAPE_INVALID, "%s: %lld tokens x %lld slots", what,
                      (long long)tokens, (long long)slots);
   const uint64_t n = (uint64_t)tokens * slots;
-  if (int rc = check_device_span(dest, n * 4, "dest")) return rc;
+  if (int rc = check_array(dest, n, 4, "dest")) return rc;
   if (source)
-    if (int rc = check_device_span(source, (uint64_t)rows * 4, "source")) return rc;
+    if (int rc = check_array(source, (uint64_t)rows, 4, "source")) return rc;
   if (weights) {
     if (int rc = check_matrix(weights, "weights", weights->type == kF32)) return rc;
     if (weights->rows != tokens || weights->cols != slots)
@@ -405,9 +405,9 @@ int dcopy_expert_sort(int32_t *dest, int32_t *source, int64_t rows, int32_t *off
   if (need && workspace_bytes < need + 16)
     return set_error(DCOPY_ERR_PARAM_INVALID, "expert_sort: workspace of %llu bytes, %llu needed",
                      (unsigned long long)workspace_bytes, (unsigned long long)need + 16);
-  if (int rc = check_device_span(dest, n * 4, "dest")) return rc;
-  if (int rc = check_device_span(source, (uint64_t)rows * 4, "source")) return rc;
-  if (int rc = check_device_span(offsets, ((uint64_t)experts + 1) * 4, "offsets")) return rc;
+  if (int rc = check_array(dest, n, 4, "dest")) return rc;
+  if (int rc = check_array(source, (uint64_t)rows, 4, "source")) return rc;
+  if (int rc = check_array(offsets, (uint64_t)experts + 1, 4, "offsets")) return rc;
   if (need)
     if (int rc = check_device_span(workspace, need + 16, "workspace")) return rc;
   // dest may be the ids themselves: an entry's id is read before its row is written, by

@@ -63,6 +63,14 @@ inline uint64_t matrix_span(const DcopyMatrix *m) {
   return ((uint64_t)(m->rows - 1) * (m->rows > 1 ? m->pitch : 0) + m->cols) * elem_size(m->type);
 }
 
+// `count` elements of a type, aligned to it.
+inline int check_array(const void *data, uint64_t count, uint64_t elem_bytes, const char *name) {
+  if (count && (uintptr_t)data % elem_bytes)
+    return set_error(DCOPY_ERR_PARAM_INVALID, "%s (%p) is not aligned to its %d-byte elements",
+                     name, data, (int)elem_bytes);
+  return check_device_span(data, count * elem_bytes, name);
+}
+
 // Whether no byte belongs to rows of both.  Rows of one pitch may interleave, as column
 // slices of one buffer do.
 inline bool apart(const DcopyMatrix *a, const DcopyMatrix *b) {

@@ -287,3 +287,28 @@ def test_layout_of_an_empty_tensor(dcopy):
     assert (rows, cols) == (6, 0)
     rows, cols, _, _ = model_ops._calls.layout(torch.zeros(6, 0).t())
     assert (rows, cols) == (0, 6)
+
+
+@pytest.mark.parametrize("op,name", [("sort", "dest"), ("sort", "source"), ("sort", "offsets"),
+                                     ("dispatch", "dest"), ("dispatch", "source"), ("combine", "dest"),
+                                     ("combine_grad", "dest"), ("combine_grad", "source")])
+def test_routing_is_aligned(dcopy, op, name):
+    """An array that does not start on its elements' alignment is refused, not read."""
+    places = places_of(dcopy, op)
+    at, *rest = places[name]
+    for off in (1, 2, 3):
+        rc, message = call_at(dcopy, op, {**places, name: (at + off, *rest)})
+        assert rc == dcopy.ERR_PARAM_INVALID and b"not aligned" in message and name.encode() in message
+
+
+def test_numbers_are_aligned(dcopy):
+    if torch.cuda.is_available():
+        pytest.skip("made-up addresses")
+    lib, built = dcopy.lib(), dcopy.DcopyGradList()
+    built.workspace = BASE
+    ref, far = ctypes.byref(built), BASE + (1 << 20)
+    for call in (lambda: lib.dcopy_grad_sum_squares(ref, far + 4, None),
+                 lambda: lib.dcopy_grad_clip(ref, far + 4, 1.0, 0.0, None, None),
+                 lambda: lib.dcopy_grad_clip(ref, far, 1.0, 0.0, far + 10, None),
+                 lambda: lib.dcopy_clip_grad_norm(ref, 1.0, 0.0, far + 2, None)):
+        assert call() == dcopy.ERR_PARAM_INVALID and b"not aligned" in lib.dcopy_last_error_message()
