@@ -357,6 +357,10 @@ int id_source(const DcopyMatrix *ids, int64_t first, int64_t keys, KeySource *sr
   const uint64_t n = (uint64_t)ids->rows * (uint64_t)ids->cols;
   if (n > INT32_MAX)
     return set_error(DCOPY_ERR_SHAPE_INVALID, "ids: %llu entries", (unsigned long long)n);
+  // Beyond this, the subtraction of first would wrap ids from the other end into the table.
+  if (keys > 0 && first > INT64_MAX - (keys - 1))
+    return set_error(DCOPY_ERR_PARAM_INVALID, "first_id %lld: the table's %lld rows pass 2^63",
+                     (long long)first, (long long)keys);
   src->ids = ids->data;
   src->pitch = ids->pitch;
   src->first = first;

@@ -21,13 +21,14 @@ struct KeySource {
   FastDiv cols;
 };
 
-// The e-th id less `first`.
+// The e-th id less `first`, modulo 2^64: with first + keys within 2^63, ids that wrap around
+// stay outside [0, keys).
 __device__ __forceinline__ int64_t read_id(const KeySource &k, uint32_t e) {
   const uint32_t r = k.cols.div(e);
   const int64_t at = (int64_t)r * k.pitch + (e - r * k.cols.d);
-  return (k.wide ? static_cast<const int64_t *>(k.ids)[at]
-                 : (int64_t)static_cast<const int32_t *>(k.ids)[at]) -
-         k.first;
+  const int64_t id = k.wide ? static_cast<const int64_t *>(k.ids)[at]
+                            : (int64_t)static_cast<const int32_t *>(k.ids)[at];
+  return (int64_t)((uint64_t)id - (uint64_t)k.first);
 }
 
 // Rows [begin, end) to zero beside the sort: its few blocks leave most SMs idle, so

@@ -525,8 +525,8 @@ typedef struct DcopyMatrix {
 
 /* out[i,:] = round(scale * table[id_i - first_id, :]), zero where id_i - first_id
  * lies outside the table (a padding id, or another rank's part of a vocabulary that
- * is split by rows).  ids: INT32 (3) or INT64 (9), read row by row; out has a row
- * for each id.  out and table may differ in type. */
+ * is split by rows; first_id + its rows within 2^63).  ids: INT32 (3) or INT64 (9),
+ * read row by row; out has a row for each id.  out and table may differ in type. */
 int dcopy_embedding_lookup(const DcopyMatrix *out, const DcopyMatrix *table,
                            const DcopyMatrix *ids, int64_t first_id, float scale,
                            dcopy_stream_t stream);

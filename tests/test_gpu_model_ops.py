@@ -698,3 +698,24 @@ def test_flat_routing_of_one_slot(torch_cuda, dcopy, n):
     assert torch.equal(dy[dest.long()], x * w)
     exact = (x.double() ** 2).sum(1, keepdim=True)
     close(dw, exact, 16, exact)
+
+
+@pytest.mark.parametrize("n", [100, 600, 5000])
+def test_ids_at_the_ends_of_the_range(torch_cuda, dcopy, n):
+    """Ids and first ids as far apart as 64 bits allow belong nowhere but where they do."""
+    top = (1 << 63) - 1
+    odd = torch.tensor([top, -top - 1, top - 1, -top, 0, -1, top - 3, -top + 2], device="cuda")
+    ids = odd[torch.arange(n, device="cuda") % 8]
+    table, dout = torch.randn(4, 8, device="cuda"), torch.randn(n, 8, device="cuda")
+    for first, rows in ((top - 3, {0: 3, 2: 2, 6: 0}), (-top - 1, {1: 0, 3: 1, 7: 3}), (-1, {4: 1, 5: 0})):
+        at = torch.full((8,), -1, device="cuda")
+        for k, row in rows.items():
+            at[k] = row
+        at = at[torch.arange(n, device="cuda") % 8]
+        out = torch.empty(n, 8, device="cuda")
+        dcopy.embedding_lookup(out, table, ids, first_id=first)
+        assert torch.equal(out, torch.where((at >= 0)[:, None], table[at.clamp(min=0)], 0.0))
+        grad = torch.empty_like(table)
+        dcopy.embedding_grad(grad, dout, ids, first_id=first)
+        exact, size = grad_exact(dout, at, 4, 1.0)
+        close(grad, exact, n, size)

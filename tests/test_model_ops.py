@@ -312,3 +312,17 @@ def test_numbers_are_aligned(dcopy):
                  lambda: lib.dcopy_grad_clip(ref, far, 1.0, 0.0, far + 10, None),
                  lambda: lib.dcopy_clip_grad_norm(ref, 1.0, 0.0, far + 2, None)):
         assert call() == dcopy.ERR_PARAM_INVALID and b"not aligned" in lib.dcopy_last_error_message()
+
+
+def test_first_ids_at_the_end_of_the_range(dcopy):
+    """A part of a vocabulary whose ids would pass 2^63 is refused: ids from the other end of
+    the range would fall into it."""
+    if torch.cuda.is_available():
+        pytest.skip("made-up addresses")
+    lib, m = dcopy.lib(), _mat(dcopy)
+    ids, out = _mat(dcopy, 0x40000, 4, 1, 1, 9), _mat(dcopy, 0x20000)
+    top = (1 << 63) - 1
+    for first, refused in ((top, True), (top - 2, True), (top - 3, False), (-top - 1, False)):
+        for rc in (lib.dcopy_embedding_lookup(out, m, ids, first, 1.0, None),
+                   lib.dcopy_embedding_grad(m, out, ids, first, 1.0, 0, 0x80000, 1 << 20, None)):
+            assert (rc == dcopy.ERR_PARAM_INVALID) == refused, (first, lib.dcopy_last_error_message())
