@@ -719,3 +719,27 @@ def test_ids_at_the_ends_of_the_range(torch_cuda, dcopy, n):
         dcopy.embedding_grad(grad, dout, ids, first_id=first)
         exact, size = grad_exact(dout, at, 4, 1.0)
         close(grad, exact, n, size)
+
+
+@pytest.mark.parametrize("n", [700, 1500, 4096, 4097, 9001])
+@pytest.mark.parametrize("vocab", [510, 511, 512, (1 << 18) - 1, 1 << 18, (1 << 18) + 1, (1 << 27) - 1, 1 << 27])
+def test_embedding_grad_where_passes_begin(torch_cuda, dcopy, vocab, n):
+    """Vocabularies on both sides of one, two, three and four passes of the sort (the key that
+    belongs nowhere is `vocab` itself, so 511 fills nine bits), of one tile and of several."""
+    g = gen(vocab + n)
+    ids = torch.randint(0, vocab, (n,), generator=g, device="cuda")
+    ids[::3] = torch.randint(max(0, vocab - 600), vocab + 1, (len(ids[::3]),), generator=g, device="cuda")
+    ids[:4] = torch.tensor([0, vocab - 1, vocab, -1], device="cuda")
+    if vocab > 1 << 20:  # wide tables: what they held stays, and only rows of tokens are looked at
+        dout, grad = randn(g, (n, 2), BF16), torch.full((vocab, 2), 2.0, device="cuda", dtype=BF16)
+        dcopy.embedding_grad(grad, dout, ids, accumulate=True)
+        known = (ids >= 0) & (ids < vocab)
+        rows, at = torch.unique(ids[known], return_inverse=True)
+        exact, size = grad_exact(dout[known], at, rows.numel(), 1.0)
+        close(grad[rows], exact + 2.0, n, size + 2.0)
+        assert int((grad != 2.0).any(1).sum()) <= rows.numel()
+        return
+    dout, grad = randn(g, (n, 8), F32), torch.empty((vocab, 8), device="cuda")
+    dcopy.embedding_grad(grad, dout, ids)
+    exact, size = grad_exact(dout, ids, vocab, 1.0)
+    close(grad, exact, n, size)
