@@ -604,9 +604,15 @@ int dcopy_expert_combine_grad(const DcopyMatrix *dy, const DcopyMatrix *dweights
     p.vectors = vectors_of(dy->cols, cut);
     p.lx = 0;
     while (p.lx < 5 && (1u << p.lx) < p.vectors) ++p.lx;
-    // A block an entry where warps alone would leave SMs idle (13 x 6 entries of 8192 fp32:
-    // 4.6 us against 9.4; 600 x 4 of 2048 bf16: 6.0 against 8.4; 1000 x 4: 13.1 against 6.4).
-    if (p.vectors >= 128 && entries <= 16ull * sm_count()) p.lx = 8;
+    // A block an entry where entries are too few for warps alone to fill the SMs.  A wide row
+    // keeps a block's threads at work, so the entries an SM grow with it.  Us with a block
+    // against a warp, on the block's side of the limit, then on the warp's: 1024 bf16, 300
+    // entries 2.1 : 2.3, 600 entries 2.9 : 2.4; 2048 bf16, 800 entries 3.5 : 3.9, 1900 entries
+    // 6.5 : 5.1; 4096 bf16, 1600 entries 7.9 : 9.5, 2200 entries 10.4 : 10.0.  Widest rows gain
+    // least at the limit: 8192 fp32, 80 entries 3.7 : 8.9, 2200 entries 28.5 : 31.7, 8000
+    // entries 97 : 103.
+    if (p.vectors >= 128 && entries <= std::min(p.vectors / 40, 16u) * (uint64_t)sm_count())
+      p.lx = 8;
     const uint64_t per_block = kRowThreads >> p.lx;
     const uint64_t blocks = p.unused_blocks + (entries + per_block - 1) / per_block;
     if (blocks == 0) return (int)DCOPY_OK;
