@@ -284,9 +284,10 @@ Routing routing(Call &c, PyObject *dest, PyObject *source, int64_t tokens, int64
                 const DcopyMatrix &weights) {
   Routing r{};
   int64_t n = 0, held = rows;
+  const at::Tensor &d = unpack(dest, "dest");
   r.dest = (const int32_t *)c.vector(dest, "dest", at::kInt, &n);
   r.source = (const int32_t *)c.vector(source, "source", at::kInt, &held);
-  if (dest != Py_None && unpack(dest, "dest").dim() > 1) r.slots = unpack(dest, "dest").size(-1);
+  if (d.dim() > 1) r.slots = d.size(-1);
   else r.slots = tokens ? n / tokens : weights.cols;
   if (r.slots * tokens != n)
     dcopy_error(DCOPY_ERR_SHAPE_INVALID, "dest has " + std::to_string(n) + " values for " +

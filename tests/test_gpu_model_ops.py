@@ -743,3 +743,16 @@ def test_embedding_grad_where_passes_begin(torch_cuda, dcopy, vocab, n):
     dcopy.embedding_grad(grad, dout, ids)
     exact, size = grad_exact(dout, ids, vocab, 1.0)
     close(grad, exact, n, size)
+
+
+def test_a_routing_is_needed(torch_cuda, dcopy):
+    """No dest is an error, not a routing without slots."""
+    x, rows = torch.ones(4, 8, device="cuda"), torch.ones(6, 8, device="cuda")
+    source, w = torch.zeros(6, dtype=torch.int32, device="cuda"), torch.ones(4, 2, device="cuda")
+    with pytest.raises(ValueError):
+        dcopy.expert_dispatch(rows, x, None, source)
+    with pytest.raises(ValueError):
+        dcopy.expert_combine(x, rows, None)
+    with pytest.raises(ValueError):
+        dcopy.expert_combine_grad(torch.empty_like(rows), w.clone(), x, rows, None, w, source)
+    assert bool((x == 1).all()) and bool((rows == 1).all())
