@@ -115,6 +115,12 @@ double as_double(PyObject *o) {
   return v;
 }
 
+bool as_bool(PyObject *o) {
+  const int v = PyObject_IsTrue(o);
+  if (v < 0) throw Raised{};
+  return v != 0;
+}
+
 // One call: its device, which all its tensors share, and its stream.
 class Call {
  public:
@@ -241,7 +247,7 @@ PyObject *embedding_grad(PyObject *, PyObject *const *a, Py_ssize_t n) {
                       ids = c.matrix(a[2], "ids");
     const float scale = (float)as_double(a[3]);
     const int64_t first = as_int(a[4]);
-    const int accumulate = PyObject_IsTrue(a[5]);
+    const int accumulate = as_bool(a[5]);
     dcopy_stream_t s = c.stream();
     uint64_t need = 0, bytes = 0;
     if (a[6] == Py_None)

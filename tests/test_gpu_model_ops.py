@@ -756,3 +756,14 @@ def test_a_routing_is_needed(torch_cuda, dcopy):
     with pytest.raises(ValueError):
         dcopy.expert_combine_grad(torch.empty_like(rows), w.clone(), x, rows, None, w, source)
     assert bool((x == 1).all()) and bool((rows == 1).all())
+
+
+def test_accumulate_is_a_truth_value(torch_cuda, dcopy):
+    """What has none raises its own error before anything is written."""
+    grad, dout = torch.ones(4, 8, device="cuda"), torch.ones(3, 8, device="cuda")
+    ids = torch.zeros(3, dtype=torch.int64, device="cuda")
+    with pytest.raises(ValueError, match="ambiguous"):
+        dcopy.embedding_grad(grad, dout, ids, accumulate=np.ones(2))
+    assert bool((grad == 1).all())
+    dcopy.embedding_grad(grad, dout, ids, accumulate=np.bool_(True))
+    assert bool((grad[0] == 4).all()) and bool((grad[1:] == 1).all())
