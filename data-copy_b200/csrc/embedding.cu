@@ -303,8 +303,9 @@ __global__ void __launch_bounds__(kRowThreads) piece_sum_kernel(Grad p) {
 
 // The runs that begin in a piece and go on: tail of that piece plus the heads of the
 // following ones, in order, kAhead of them fetched before it is known how many count.
-// Bound by the latency of the longest run (an id that 6 % of 16384 tokens have: 17 us),
-// which the zeroing beside it hides.
+// Bound by the latency of the longest run, one thread a column over all its pieces (1024
+// columns, an id that 6 % of 65536 tokens have: 27 us, of 262144: 93); the zeroing of a
+// large table beside it hides that, nothing does when gradients accumulate.
 template <typename TOut, int V, bool kAdd>
 __global__ void __launch_bounds__(kRowThreads, 4) piece_join_kernel(Grad p) {
   pdl_trigger_at_entry();

@@ -601,8 +601,9 @@ int dcopy_grad_list_build(DcopyGradList *list, const DcopyGrad *grads, uint32_t 
 int dcopy_grad_sum_squares(const DcopyGradList *list, double *total, dcopy_stream_t stream);
 /* norm = sqrt(total[0]); dst = round(c * src) with c = min(1, max_norm / (norm + eps)).
  * norm (device, fp32; NULL: not written) gets the norm.  A rank that holds a part of
- * the gradients adds up the totals of all ranks between the two calls.  A norm that is
- * infinite or NaN goes into c as the formula has it. */
+ * the gradients adds up the totals of all ranks between the two calls.  The norm is
+ * held in fp32: above its range it is infinite.  A norm that is infinite or NaN goes into
+ * c as the formula has it. */
 int dcopy_grad_clip(const DcopyGradList *list, const double *total, float max_norm, float eps,
                     float *norm, dcopy_stream_t stream);
 /* Both in turn, for gradients that are all here. */
