@@ -132,3 +132,29 @@ def test_a_list_lives_on_the_stream_it_is_built_on(dcopy, fresh_stream):
     norm = torch.empty(1, device="cuda")
     dcopy.clip_grad_norm(held, 1.0, norm)
     assert abs(norm.item() - 1000 ** 0.5) <= 40 * 2.0 ** -24 * 1000 ** 0.5
+
+
+def test_given_streams_inside_a_graph(torch_cuda, dcopy):
+    """A captured step that forks to a stream of its own: workspaces come from the graph's
+    memory, and a list used there stays usable outside."""
+    outs, run = calls(dcopy)
+    grads = [torch.randn(5000, device="cuda"), torch.randn(77, device="cuda")]
+    clipped, norm = [torch.empty_like(g) for g in grads], torch.empty(1, device="cuda")
+    held = dcopy.GradList(grads, clipped)
+    run()
+    dcopy.clip_grad_norm(held, 1.0, norm)
+    everything = outs + clipped + [norm]
+    want = [t.clone() for t in everything]
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        side.wait_stream(torch.cuda.current_stream())
+        run(side)
+        dcopy.clip_grad_norm(held, 1.0, norm, stream=side)
+        torch.cuda.current_stream().wait_stream(side)
+    for t in everything:
+        t.fill_(-7)
+    graph.replay()
+    assert all(torch.equal(a, b) for a, b in zip(want, everything))
+    norm.zero_()
+    dcopy.clip_grad_norm(held, 1.0, norm)
+    assert torch.equal(norm, want[-1])
